@@ -48,6 +48,13 @@ PAIR_BIAS_NONE = 0
 PAIR_BIAS_NORMALIZED_INPUT = 1
 PAIR_BIAS_SEPARATE = 2
 
+ROTARY_HALF = 0
+ROTARY_INTERLEAVED = 1
+
+HEAD_NORM_NONE = 0
+HEAD_NORM_RMS = 1
+HEAD_NORM_LAYER = 2
+
 
 class AfhipUnavailable(RuntimeError):
     """libafhip.so is not built or cannot be loaded; nothing falls back."""
@@ -114,6 +121,29 @@ class AttentionDesc(ctypes.Structure):
         ("heads", ctypes.c_int32), ("transpose", ctypes.c_int32), ("pair_bias", ctypes.c_int32),
         ("pair_channels", ctypes.c_int32), ("precision", ctypes.c_int32), ("in_dtype", ctypes.c_int32),
         ("out_dtype", ctypes.c_int32), ("residual", ctypes.c_int32), ("epsilon", ctypes.c_float),
+    ]
+
+
+class Strides(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int64), ("token", ctypes.c_int64), ("head", ctypes.c_int64)]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32), ("query_heads", ctypes.c_int32),
+        ("key_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32),
+        ("layout", ctypes.c_int32), ("norm", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("capacity", ctypes.c_int32), ("epsilon", ctypes.c_float), ("rotation_scale", ctypes.c_float),
+        ("q", Strides), ("k", Strides), ("v", Strides), ("q_out", Strides), ("k_out", Strides), ("v_out", Strides),
+    ]
+
+
+class WindowDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("queries", ctypes.c_int32), ("keys", ctypes.c_int32),
+        ("query_heads", ctypes.c_int32), ("key_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("left", ctypes.c_int32), ("right", ctypes.c_int32), ("sinks", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("q", Strides), ("k", Strides), ("v", Strides), ("out", Strides),
     ]
 
 
@@ -191,6 +221,14 @@ SIGNATURES = {
     "afhip_attention_workspace_size": [ctypes.POINTER(AttentionDesc), _szp],
     "afhip_attention_prepare_weights": [ctypes.POINTER(AttentionDesc), _vp, _vp, _vp],
     "afhip_attention_run": [ctypes.POINTER(AttentionDesc), _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
+    "afhip_rotary_run": [ctypes.POINTER(RotaryDesc)] + [_vp] * 15,
+    "afhip_rotary_backward_workspace_size": [ctypes.POINTER(RotaryDesc), _szp],
+    "afhip_rotary_backward": [ctypes.POINTER(RotaryDesc)] + [_vp] * 17 + [_sz, _vp],
+    "afhip_window_workspace_size": [ctypes.POINTER(WindowDesc), _szp],
+    "afhip_window_run": [ctypes.POINTER(WindowDesc)] + [_vp] * 8 + [_sz, _vp],
+    "afhip_window_backward_workspace_size": [ctypes.POINTER(WindowDesc), _szp],
+    "afhip_window_backward": [ctypes.POINTER(WindowDesc)] + [_vp] * 6 + [ctypes.POINTER(Strides)] + [_vp] * 6 +
+                             [_sz, _vp],
     "afhip_set_memory_budget": [ctypes.c_uint64],
     "afhip_memory_resident": [ctypes.POINTER(ctypes.c_uint64)],
     "afhip_execution_create": [ctypes.c_uint64, _vp, ctypes.POINTER(_vp)],

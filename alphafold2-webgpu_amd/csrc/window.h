@@ -1,0 +1,192 @@
+// What the kernels of the windowed attention share (window.hip,
+// window_backward.hip): the arguments, which keys a query sees, and tiles of
+// rows in LDS with the fragments the MFMA takes from them.
+#pragma once
+
+#include "dma.h"
+#include "heads.h"
+
+namespace afhip {
+
+constexpr float kWindowLog2e = 1.4426950408889634f;
+constexpr float kWindowLn2 = 0.6931471805599453f;
+
+struct WindowArgs {
+  const char *q, *k, *v;
+  char* out;
+  float* lse;
+  const int32_t *query_lengths, *key_lengths;
+  float* partial;  // split keys: [row][split] of head_dim sums, the reference point, the total
+  HeadStrides sq, sk, sv, so;
+  int batch, queries, keys, query_heads, key_heads, group, head_dim;
+  int left, right, sinks;
+  float scale, scale_log2;
+  int tiles, splits;
+  // The way back.
+  const char *o, *dout;
+  HeadStrides sdo;
+  char *dq, *dk, *dv;
+  // [batch][key head][row]: the row's lse in base 2 and the sum of out * dout; the keys it sees, below and from.
+  float2* rows;
+  int2* limits;
+};
+
+typedef float floatx8 __attribute__((ext_vector_type(8)));
+typedef short window_short4 __attribute__((ext_vector_type(4)));
+typedef short window_short8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) window_short4 lds_window_short4;
+
+// Eight values along a product's inner axis, a lane's part of 16.
+template <typename T> struct Eight;
+template <> struct Eight<half_t> { typedef half8 type; };
+template <> struct Eight<float> { typedef floatx8 type; };
+
+// acc[32 x 32] += A[32 x 16] B[16 x 32]. Element j of the lane's eight pairs with element j of B's in the same half of
+// the wave; in f32, one MFMA of inner length 2 for each j (a value of each half).
+__device__ __forceinline__ floatx16 mma(half8 a, half8 b, floatx16 c) { return mfma_f16(a, b, c); }
+__device__ __forceinline__ floatx16 mma(floatx8 a, floatx8 b, floatx16 c) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) c = mfma_f32(a[j], b[j], c);
+  return c;
+}
+
+// Rows of DP channels (zeros past head_dim) in LDS, 16-byte chunks XORed with their row so that the reads of one
+// column of chunks (nat) and of a few rows (tr) spread over the banks.
+template <typename T, int DP> struct Tile {
+  typedef typename Eight<T>::type Frag;
+  static constexpr int kRow = DP * (int)sizeof(T), kChunks = kRow / 16;
+
+  static __device__ __forceinline__ int swizzle(int row) { return kChunks >= 8 ? row & 7 : (row >> 1) & 3; }
+
+  // Channels 16 kk + 8 (lane / 32) .. + 8 of row `row`.
+  static __device__ __forceinline__ Frag nat(const unsigned char* t, int row, int kk, int hi) {
+    const unsigned char* p = t + row * kRow;
+    const int sw = swizzle(row);
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const half8*>(p + 16 * ((2 * kk + hi) ^ sw));
+    } else {
+      const floatx4 a = *reinterpret_cast<const floatx4*>(p + 16 * ((4 * kk + 2 * hi) ^ sw));
+      const floatx4 b = *reinterpret_cast<const floatx4*>(p + 16 * ((4 * kk + 2 * hi + 1) ^ sw));
+      return floatx8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+  }
+
+  // Channel 32 cb + lane % 32 of rows row0 + 4 (lane / 32) + {0..3} and those + 8: the rows that the lane's eight
+  // accumulators 8 s .. of a product have (mfma_row), row0 = 16 s. In f16 two transposing reads.
+  static __device__ __forceinline__ Frag tr(const unsigned char* t, int row0, int cb, int lane) {
+    const int hi = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int row = row0 + 4 * hi + ((lane & 15) >> 2);
+      const int ch = 32 * cb + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      const unsigned char* p = t + row * kRow + 16 * ((ch >> 3) ^ swizzle(row)) + 2 * (ch & 7);
+      const window_short4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_window_short4*)p);
+      const window_short4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_window_short4*)(p + 8 * kRow));
+      return __builtin_bit_cast(half8, window_short8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+    } else {
+      const int ch = 32 * cb + (lane & 31);
+      Frag f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int row = row0 + 4 * hi + (j & 3) + 8 * (j >> 2);
+        f[j] = *reinterpret_cast<const float*>(t + row * kRow + 16 * ((ch >> 2) ^ swizzle(row)) + 4 * (ch & 3));
+      }
+      return f;
+    }
+  }
+};
+
+// What a wave loads of a tile of ROWS rows, shared among WAVES waves: which row and byte each lane's chunk of each
+// instruction comes from.
+template <typename T, int DP, int ROWS, int WAVES> struct TileLoad {
+  static constexpr int kChunks = Tile<T, DP>::kChunks, kCount = ROWS * kChunks / 64 / WAVES;
+  static constexpr int kBytes = ROWS * DP * (int)sizeof(T);
+  static_assert(ROWS * kChunks % (64 * WAVES) == 0, "whole instructions for each wave");
+
+  static constexpr int kStep = 64 / kChunks;  // rows of an instruction
+  static constexpr int kUnroll = kCount > 8 ? 2 : kCount;
+  int row, chunk, chunks;                     // the lane's row and chunk in a wave's first; a row's chunks
+
+  __device__ __forceinline__ void init(int wave, int lane, int head_dim) {
+    row = kStep * wave + lane / kChunks;
+    chunk = lane % kChunks;
+    chunks = head_dim * (int)sizeof(T) / 16;
+  }
+
+  // Rows row0 .. of the tensor at `base`, those that keep(row) holds for; zeros for the others. At most 64 rows of
+  // token strides up to 2^24 bytes: offsets stay below 2^30.
+  template <typename Keep>
+  __device__ __forceinline__ void issue(const char* base, int64_t token, int row0, uint32_t lds, int wave,
+                                        Keep keep) const {
+    const int32x4_t rsrc = make_rsrc(base + (int64_t)row0 * token, 0x7ffffff0u);
+#pragma unroll kUnroll
+    for (int n = 0; n < kCount; n++) {
+      const int r = row + kStep * WAVES * n, c = chunk ^ Tile<T, DP>::swizzle(r);
+      const bool ok = (c < chunks) & keep(row0 + r);
+      dma16(rsrc, lds + 1024 * (wave + WAVES * n), ok ? (uint32_t)r * (uint32_t)token + 16u * c : kOutOfRange);
+    }
+  }
+};
+
+// Eight channels of a row in global memory; zeros where there are none.
+template <typename T> __device__ __forceinline__ typename Eight<T>::type load_eight(const char* row, int channel,
+                                                                                    bool keep) {
+  typename Eight<T>::type f{};
+  if (keep) f = *reinterpret_cast<const typename Eight<T>::type*>(row + channel * (int)sizeof(T));
+  return f;
+}
+
+// Eight accumulators as the second operand of the next product.
+__device__ __forceinline__ half8 pack8(const float* x, half8*) {
+  half8 f;
+#pragma unroll
+  for (int j = 0; j < 8; j++) f[j] = (half_t)x[j];
+  return f;
+}
+__device__ __forceinline__ floatx8 pack8(const float* x, floatx8*) {
+  return floatx8{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+}
+
+// One sequence: its numbers of queries and keys, and where its queries start.
+struct Sequence {
+  int queries, keys, offset;
+  __device__ __forceinline__ Sequence(const WindowArgs& a, int b) {
+    queries = a.query_lengths ? min(max(a.query_lengths[b], 0), a.queries) : a.queries;
+    keys = a.key_lengths ? min(max(a.key_lengths[b], 0), a.keys) : a.keys;
+    offset = keys - queries;
+  }
+  // Keys [low, high) and those below min(sinks, high) are what query i sees.
+  __device__ __forceinline__ int high(const WindowArgs& a, int i) const {
+    return a.right < 0 ? keys : min(keys, max(0, offset + i + a.right + 1));
+  }
+  __device__ __forceinline__ int low(const WindowArgs& a, int i) const {
+    return a.left < 0 ? 0 : max(0, offset + i - a.left);
+  }
+};
+
+// Whether a row that sees keys [low, high) and those below min(sinks, high) does not see `key`: one comparison, so
+// that a block's sixteen tests do not fill the scalar registers with masks.
+__device__ __forceinline__ bool hidden(int key, int low, int high, int sinks) {
+  return min(max(low - key, key - (high - 1)), key - (min(sinks, high) - 1)) > 0;
+}
+
+// The blocks of BK keys that queries first .. last of a sequence see: `sink_blocks` at the start, then `blocks` from
+// `start` on.
+struct KeyRange {
+  int low, high, sinks, sink_blocks, start, total;
+  __device__ __forceinline__ KeyRange(const WindowArgs& a, const Sequence& s, int first, int last, int BK) {
+    high = s.high(a, last);
+    low = min(s.low(a, first), high);
+    sinks = a.left < 0 ? 0 : min(a.sinks, high);
+    start = low / BK;
+    sink_blocks = min((sinks + BK - 1) / BK, start);
+    const int end = (high + BK - 1) / BK;
+    total = sink_blocks + (low < high || sinks > start * BK ? end - start : 0);
+  }
+  __device__ __forceinline__ int block(int t) const { return t < sink_blocks ? t : start + t - sink_blocks; }
+  __device__ __forceinline__ bool keeps(int key) const { return (key < high) & ((key >= low) | (key < sinks)); }
+};
+
+int window_check(const afhip_window_desc* desc);
+void window_fill(const afhip_window_desc& d, WindowArgs& a);
+
+}  // namespace afhip

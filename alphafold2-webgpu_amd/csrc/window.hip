@@ -1,0 +1,519 @@
+// Attention over a window of keys and the first few ("sinks"), for prompts and
+// for single tokens against a cache:
+//
+//   p = key_length - query_length + i;  key j is seen iff j < key_length, j <= p + right, and j >= p - left or j < sinks
+//   out = sum_j e^(s_j - m) v_j / l,  l = sum_j e^(s_j - m),  lse = m + ln l,  s_j = scale q . k_j
+//
+// in one pass over the keys with a running reference point m. Query heads that
+// share a key head are rows of one tile: row r of a key head is query r / group
+// of head r % group, so that a tile reads each key once for all of them.
+//
+// Both products run on the MFMA as S^T = K Q^T and O^T = V^T P^T: a lane then
+// holds one row's scores for 16 keys and the same row's output for 16 channels,
+// the reference point and the sum stay inside the lane (and the lane 32 away),
+// and the probabilities feed the second product from the registers they were
+// computed in. K and V go to LDS by DMA; V^T comes from gfx950's transposing LDS
+// read. f32 runs the same on the f32 MFMA.
+//
+// Blocks of keys that no query of a workgroup sees are not visited, rows of one
+// that none sees are loaded as zeros (whatever is there, infinities and NaN too),
+// and the comparisons run only in blocks that some row sees in part.
+#include <algorithm>
+#include <cmath>
+
+#include "window.h"
+
+namespace afhip {
+
+namespace {
+
+// A probability is held as 2^(x - m + kLift), in f16 within 2^-24 and 2^(kLift + kSlack): the reference point m moves
+// only when a score passes it by more than kSlack, and small probabilities of long rows keep their bits.
+template <typename T> constexpr float kLift = sizeof(T) == 2 ? 6.0f : 0.0f;
+constexpr float kSlack = 8.0f;
+
+// One wave's 32 rows: Q, the running state and the output so far.
+template <typename T, int DP> struct Rows {
+  typedef typename Eight<T>::type Frag;
+  static constexpr int kSteps = DP / 16, kBlocks = DP / 32;
+  Frag q[kSteps];
+  floatx16 o[kBlocks];
+  float m, l;
+  int high, low;  // what this lane's row sees
+
+  __device__ __forceinline__ void init(const WindowArgs& a, const Sequence& s, int b, int kv, int row, int hi) {
+    const int i = row / a.group, h = kv * a.group + row % a.group;
+    const bool live = i < s.queries;
+    const char* p = a.q + b * a.sq.batch + (int64_t)(live ? i : 0) * a.sq.token + h * a.sq.head;
+#pragma unroll
+    for (int kk = 0; kk < kSteps; kk++) {
+      const int ch = 16 * kk + 8 * hi;
+      q[kk] = load_eight<T>(p, ch, live && ch < a.head_dim);
+    }
+#pragma unroll
+    for (int c = 0; c < kBlocks; c++) o[c] = floatx16{};
+    m = -INFINITY;
+    l = 0.0f;
+    // A row past the length counts as the last one (its results are dropped), so that it makes no block partial.
+    const int at = min(i, s.queries - 1);
+    high = s.high(a, at);
+    low = s.low(a, at);
+  }
+
+  // 32 NB keys from k0 on: K and V tiles at kt and vt, `partial` where some row does not see all of them.
+  template <int NB>
+  __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int k0, bool partial,
+                                       int sinks, float scale, int lane) {
+    const int col = lane & 31, hi = lane >> 5;
+    floatx16 x[NB];
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      x[n] = floatx16{};
+#pragma unroll
+      for (int kk = 0; kk < kSteps; kk++) x[n] = mma(Tile<T, DP>::nat(kt, 32 * n + col, kk, hi), q[kk], x[n]);
+    }
+    if (partial) {
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+          const int key = k0 + 32 * n + mfma_row(v, lane);
+          if (hidden(key, low, high, sinks)) x[n][v] = -INFINITY;
+        }
+    }
+    float top = x[0][0];
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) top = fmaxf(top, x[n][v]);
+    top *= scale;
+    if (__builtin_amdgcn_ballot_w64(top > m + kSlack)) {
+      const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+      const float f = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+      l *= f;
+#pragma unroll
+      for (int c = 0; c < kBlocks; c++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) o[c][v] *= f;
+      m = to;
+    }
+    const float offset = kLift<T> - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      float p[16];
+#pragma unroll
+      for (int v = 0; v < 16; v++) p[v] = __builtin_amdgcn_exp2f(fmaf(x[n][v], scale, offset));
+      l += (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
+           (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        const Frag f = pack8(p + 8 * s, (Frag*)nullptr);
+#pragma unroll
+        for (int c = 0; c < kBlocks; c++) o[c] = mma(Tile<T, DP>::tr(vt, 32 * n + 16 * s, c, lane), f, o[c]);
+      }
+    }
+  }
+};
+
+// Writes four channels.
+__device__ __forceinline__ void put4(half_t* p, float a, float b, float c, float d) {
+  *reinterpret_cast<half4*>(p) = half4{(half_t)a, (half_t)b, (half_t)c, (half_t)d};
+}
+__device__ __forceinline__ void put4(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<floatx4*>(p) = floatx4{a, b, c, d};
+}
+
+// The natural logarithm of a row's sum, from its reference point and total (both in base 2).
+template <typename T> __device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.0f ? -INFINITY : (m - kLift<T> + log2f(l)) * kWindowLn2;
+}
+
+__device__ __forceinline__ int64_t lse_index(const WindowArgs& a, int b, int h, int i) {
+  return ((int64_t)b * a.query_heads + h) * a.queries + i;
+}
+
+// Four waves of 32 rows over blocks of BK keys that they share through two buffers.
+constexpr int kWaves = 4, kTileRows = 32 * kWaves;
+template <typename T> constexpr int kBlockKeys = sizeof(T) == 2 ? 64 : 32;
+
+template <typename T, int DP, bool SPLIT>
+__global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void window_rows_kernel(WindowArgs a) {
+  constexpr int BK = kBlockKeys<T>;
+  typedef TileLoad<T, DP, BK, kWaves> Load;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Neighbours are other key heads (with 8 of them or a multiple, a head's workgroups share an XCD's L2), the last
+  // rows first: without a window they see the most keys.
+  const int heads = a.batch * a.key_heads;
+  const int pair = blockIdx.x % heads, rest = blockIdx.x / heads;
+  const int b = pair / a.key_heads, kv = pair % a.key_heads;
+  const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
+  const Sequence s(a, b);
+  const int rows = a.queries * a.group;
+  const int r0 = tile * kTileRows, row = r0 + 32 * wave + (lane & 31);
+  const int first = r0 / a.group, last = min(s.queries - 1, (r0 + kTileRows - 1) / a.group);
+
+  Rows<T, DP> st;
+  st.init(a, s, b, kv, row, hi);
+  if (first < s.queries) {
+    const KeyRange range(a, s, first, last, BK);
+    const int begin = SPLIT ? (int)((int64_t)range.total * split / a.splits) : 0;
+    const int end = SPLIT ? (int)((int64_t)range.total * (split + 1) / a.splits) : range.total;
+    // What the wave's rows all see, and what any of them sees.
+    const int wr0 = r0 + 32 * wave;
+    const int wfirst = min(wr0 / a.group, s.queries - 1), wlast = min((wr0 + 31) / a.group, s.queries - 1);
+    const int all_low = s.low(a, wlast), all_high = s.high(a, wfirst);
+    const int any_low = s.low(a, wfirst), any_high = s.high(a, wlast);
+    const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
+    const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
+    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
+    Load load;
+    load.init(wave, lane, a.head_dim);
+    auto issue = [&](int t) {
+      const int k0 = range.block(t) * BK;
+      const uint32_t buffer = lds + (uint32_t)((t - begin) & 1) * 2 * Load::kBytes;
+      auto keep = [&](int key) { return range.keeps(key); };
+      load.issue(kb, a.sk.token, k0, buffer, wave, keep);
+      load.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, keep);
+    };
+    if (begin < end) issue(begin);
+    for (int t = begin; t < end; t++) {
+      // Block t is the only one in flight; the barrier publishes it, and every wave is done with block t - 1.
+      wait_vmcnt<0>();
+      block_barrier();
+      if (t + 1 < end) issue(t + 1);
+      const int k0 = range.block(t) * BK;
+      if (wr0 >= s.queries * a.group || k0 >= any_high || (k0 + BK <= any_low && k0 >= range.sinks)) continue;
+      const bool partial = k0 + BK > all_high || (k0 < all_low && k0 + BK > range.sinks);
+      const unsigned char* kt = smem + ((t - begin) & 1) * 2 * Load::kBytes;
+      st.template step<BK / 32>(kt, kt + Load::kBytes, k0, partial, range.sinks, a.scale_log2, lane);
+    }
+  }
+  const float l = st.l + __shfl_xor(st.l, 32);
+  if (row >= rows) return;
+  const int i = row / a.group, h = kv * a.group + row % a.group;
+  if constexpr (SPLIT) {
+    const int64_t n = ((int64_t)pair * rows + row) * a.splits + split;
+    float* to = a.partial + n * (a.head_dim + 2);
+#pragma unroll
+    for (int c = 0; c < DP / 32; c++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int ch = 32 * c + 8 * g + 4 * hi;
+        if (ch >= a.head_dim) continue;
+#pragma unroll
+        for (int j = 0; j < 4; j++) to[ch + j] = st.o[c][4 * g + j];
+      }
+    if (!hi) to[a.head_dim] = st.m, to[a.head_dim + 1] = l;
+  } else {
+    const bool live = i < s.queries && l != 0.0f;
+    const float inv = 1.0f / l;
+    T* to = reinterpret_cast<T*>(a.out + b * a.so.batch + i * a.so.token + h * a.so.head);
+#pragma unroll
+    for (int c = 0; c < DP / 32; c++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int ch = 32 * c + 8 * g + 4 * hi;
+        if (ch >= a.head_dim) continue;
+        const floatx16& o = st.o[c];
+        if (live) {
+          put4(to + ch, o[4 * g] * inv, o[4 * g + 1] * inv, o[4 * g + 2] * inv, o[4 * g + 3] * inv);
+        } else {
+          put4(to + ch, 0.0f, 0.0f, 0.0f, 0.0f);
+        }
+      }
+    if (a.lse && !hi) a.lse[lse_index(a, b, h, i)] = live ? row_lse<T>(st.m, l) : -INFINITY;
+  }
+}
+
+// At most 32 rows of a key head (single tokens, or few of them): its waves take blocks of 32 keys in turn, each through
+// buffers of its own, with no barrier until the end, where their sums meet in LDS. What bounds it is the cache's
+// bytes; a split adds workgroups until they fill the card.
+template <typename T, int DP> struct Step {
+  static constexpr int kBytes = 2 * 32 * DP * (int)sizeof(T);  // K and V of a block
+  static constexpr int kWaves = kBytes >= 32768 ? 2 : 4;
+  static constexpr int kStages = kBytes >= 16384 ? 2 : 4;
+  static constexpr int kLds = kWaves * kStages * kBytes;
+  static_assert(kLds >= kWaves * 32 * (DP + 2) * 4, "the waves' sums fit");
+};
+
+template <typename T, int DP> constexpr int kStepThreads = 64 * Step<T, DP>::kWaves;
+
+template <typename T, int DP>
+__global__ __launch_bounds__((kStepThreads<T, DP>)) void window_step_kernel(WindowArgs a) {
+  typedef Step<T, DP> S;
+  constexpr int W = S::kWaves, STAGES = S::kStages;
+  typedef TileLoad<T, DP, 32, 1> Load;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = a.batch * a.key_heads;
+  const int pair = blockIdx.x % heads, split = blockIdx.x / heads;
+  const int b = pair / a.key_heads, kv = pair % a.key_heads;
+  const Sequence s(a, b);
+  const int rows = a.queries * a.group;
+  Rows<T, DP> st;
+  st.init(a, s, b, kv, min(col, rows - 1), hi);
+  if (s.queries > 0) {
+    const KeyRange range(a, s, 0, s.queries - 1, 32);
+    const int begin = (int)((int64_t)range.total * split / a.splits);
+    const int end = (int)((int64_t)range.total * (split + 1) / a.splits);
+    const int all_low = s.low(a, s.queries - 1), all_high = s.high(a, 0);
+    const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
+    const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
+    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem) + wave * STAGES * S::kBytes;
+    Load load;
+    load.init(0, lane, a.head_dim);
+    const int mine = begin + wave < end ? (end - begin - wave + W - 1) / W : 0;
+    auto issue = [&](int n) {
+      const int k0 = range.block(begin + wave + n * W) * 32;
+      const uint32_t buffer = lds + (uint32_t)(n % STAGES) * S::kBytes;
+      auto keep = [&](int key) { return range.keeps(key); };
+      load.issue(kb, a.sk.token, k0, buffer, 0, keep);
+      load.issue(vb, a.sv.token, k0, buffer + S::kBytes / 2, 0, keep);
+    };
+    for (int n = 0; n < STAGES - 1 && n < mine; n++) issue(n);
+    for (int n = 0; n < mine; n++) {
+      // The buffer that block n + STAGES - 1 goes to was read by step n - 1, whose reads have returned.
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (n + STAGES - 1 < mine) {
+        issue(n + STAGES - 1);
+        wait_vmcnt<2 * Load::kCount * (STAGES - 1)>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      const int k0 = range.block(begin + wave + n * W) * 32;
+      const bool partial = k0 + 32 > all_high || (k0 < all_low && k0 + 32 > range.sinks);
+      const unsigned char* kt = smem + (wave * STAGES + n % STAGES) * S::kBytes;
+      st.template step<1>(kt, kt + S::kBytes / 2, k0, partial, range.sinks, a.scale_log2, lane);
+    }
+  }
+  // The waves' reference points, totals and sums: [wave][row][m, l, DP sums].
+  float* sums = reinterpret_cast<float*>(smem);
+  const float l = st.l + __shfl_xor(st.l, 32);
+  block_barrier();  // every wave's loads have landed and been read
+  constexpr int PITCH = DP + 2;
+  float* mine = sums + (wave * 32 + col) * PITCH;
+  if (col < rows) {
+    if (!hi) mine[0] = st.m, mine[1] = l;
+#pragma unroll
+    for (int c = 0; c < DP / 32; c++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) mine[2 + 32 * c + mfma_row(v, lane)] = st.o[c][v];
+  }
+  block_barrier();
+  for (int n = threadIdx.x; n < rows * DP; n += 64 * W) {
+    const int r = n / DP, ch = n % DP;
+    if (ch >= a.head_dim) continue;
+    float m = -INFINITY, total = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; w++) m = fmaxf(m, sums[(w * 32 + r) * PITCH]);
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      const float* p = sums + (w * 32 + r) * PITCH;
+      const float f = p[0] == m ? 1.0f : __builtin_amdgcn_exp2f(p[0] - m);
+      total += f * p[1];
+      o += f * p[2 + ch];
+    }
+    const int i = r / a.group, h = kv * a.group + r % a.group;
+    if (a.splits > 1) {
+      float* to = a.partial + (((int64_t)pair * rows + r) * a.splits + split) * (a.head_dim + 2);
+      to[ch] = o;
+      if (ch == 0) to[a.head_dim] = m, to[a.head_dim + 1] = total;
+    } else {
+      const bool live = i < s.queries;
+      T* to = reinterpret_cast<T*>(a.out + b * a.so.batch + i * a.so.token + h * a.so.head);
+      to[ch] = (T)(live && total != 0.0f ? o / total : 0.0f);
+      if (ch == 0 && a.lse) a.lse[lse_index(a, b, h, i)] = live ? row_lse<T>(m, total) : -INFINITY;
+    }
+  }
+}
+
+// Joins the splits of a row, one wave a row and two channels a lane.
+template <typename T> __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (int64_t)a.queries * a.group;
+  if (n >= (int64_t)a.batch * a.key_heads * rows) return;
+  const int pair = (int)(n / rows), row = (int)(n % rows);
+  const int b = pair / a.key_heads, kv = pair % a.key_heads, i = row / a.group, h = kv * a.group + row % a.group;
+  const Sequence s(a, b);
+  const float* from = a.partial + n * a.splits * (a.head_dim + 2);
+  const float* at = from + (int64_t)min(lane, a.splits - 1) * (a.head_dim + 2) + a.head_dim;
+  const float mine = lane < a.splits ? at[0] : -INFINITY;
+  float m = mine;
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) m = fmaxf(m, __shfl_xor(m, step));
+  const float f = mine == m ? 1.0f : __builtin_amdgcn_exp2f(mine - m);
+  float total = lane < a.splits ? f * at[1] : 0.0f;
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) total += __shfl_xor(total, step);
+  float o[2] = {0.0f, 0.0f};
+  for (int k = 0; k < a.splits; k++) {
+    const float w = __shfl(f, k);
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      if (lane + 64 * j < a.head_dim) o[j] += w * from[(int64_t)k * (a.head_dim + 2) + lane + 64 * j];
+  }
+  const bool live = i < s.queries && total != 0.0f;
+  T* to = reinterpret_cast<T*>(a.out + b * a.so.batch + i * a.so.token + h * a.so.head);
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+    if (lane + 64 * j < a.head_dim) to[lane + 64 * j] = (T)(live ? o[j] / total : 0.0f);
+  if (lane == 0 && a.lse) a.lse[lse_index(a, b, h, i)] = live ? row_lse<T>(m, total) : -INFINITY;
+}
+
+// Which kernel a call takes, and into how many parts its keys are split.
+struct Plan {
+  bool step;
+  int tiles, splits;
+};
+
+constexpr int kMaxSplits = 64;  // a lane each in window_join_kernel
+
+Plan plan(const afhip_window_desc& d) {
+  const int64_t group = d.query_heads / d.key_heads, rows = d.queries * group, heads = (int64_t)d.batch * d.key_heads;
+  Plan p{};
+  p.step = rows <= 32;
+  p.tiles = p.step ? 1 : (int)ceil_div(rows, kTileRows);
+  // The most keys that a tile's queries see.
+  int64_t span = d.keys;
+  if (d.left >= 0) {
+    const int64_t queries = p.step ? d.queries : std::min<int64_t>(d.queries, ceil_div(kTileRows, group) + 1);
+    const int64_t right = d.right < 0 ? d.keys : d.right;
+    span = std::min(span, (int64_t)d.left + right + queries + std::min<int64_t>(d.sinks, d.keys));
+  }
+  const int64_t blocks = ceil_div(span, 32), groups = heads * p.tiles;
+  // Workgroups for every CU, each with a few blocks of keys left.
+  const int64_t wanted = p.step ? 512 : 512, least = p.step ? 16 : 16;
+  int64_t splits = std::min(ceil_div(wanted, groups), blocks / least);
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
+  return p;
+}
+
+size_t partial_bytes(const afhip_window_desc& d, const Plan& p) {
+  if (p.splits == 1) return 0;
+  return (size_t)d.batch * d.queries * d.query_heads * p.splits * (d.head_dim + 2) * sizeof(float);
+}
+
+template <typename T, int DP> int launch_forward(const WindowArgs& a, const Plan& p, hipStream_t st) {
+  int s;
+  const int64_t groups = (int64_t)a.batch * a.key_heads * p.tiles * p.splits;
+  AFHIP_REQUIRE(groups < ((int64_t)1 << 31), "attention grid too large");
+  if (p.step) {
+    typedef Step<T, DP> S;
+    auto k = window_step_kernel<T, DP>;
+    if ((s = allow_lds((const void*)k, S::kLds))) return s;
+    s = launch("window.step", k, dim3((unsigned)groups), dim3(64 * S::kWaves), S::kLds, st, a);
+  } else {
+    constexpr size_t lds = 4 * kBlockKeys<T> * DP * sizeof(T);
+    auto k = p.splits > 1 ? window_rows_kernel<T, DP, true> : window_rows_kernel<T, DP, false>;
+    if ((s = allow_lds((const void*)k, lds))) return s;
+    s = launch("window.rows", k, dim3((unsigned)groups), dim3(64 * kWaves), lds, st, a);
+  }
+  if (s || p.splits == 1) return s;
+  const int64_t rows = (int64_t)a.batch * a.queries * a.query_heads;
+  AFHIP_REQUIRE(ceil_div(rows, 4) < ((int64_t)1 << 31), "attention grid too large");
+  return launch("window.join", window_join_kernel<T>, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a);
+}
+
+template <typename T> int launch_width(const WindowArgs& a, const Plan& p, hipStream_t st) {
+  if (a.head_dim <= 32) return launch_forward<T, 32>(a, p, st);
+  if (a.head_dim <= 64) return launch_forward<T, 64>(a, p, st);
+  return launch_forward<T, 128>(a, p, st);
+}
+
+}  // namespace
+
+int window_check(const afhip_window_desc* desc) {
+  AFHIP_REQUIRE(desc != nullptr, "descriptor is NULL");
+  const afhip_window_desc& d = *desc;
+  AFHIP_REQUIRE(d.batch > 0 && d.queries > 0 && d.keys > 0 && d.query_heads > 0 && d.key_heads > 0 && d.head_dim > 0,
+                "attention dimensions must be positive");
+  AFHIP_REQUIRE(d.head_dim % 8 == 0 && d.head_dim <= kMaxHeadDim, "head dimension %d is not a multiple of 8 up to %d",
+                d.head_dim, kMaxHeadDim);
+  AFHIP_REQUIRE(d.query_heads % d.key_heads == 0, "%d query heads over %d key heads", d.query_heads, d.key_heads);
+  AFHIP_REQUIRE(d.left >= -1 && d.right >= -1 && d.sinks >= 0, "left and right are at least -1, sinks at least 0");
+  AFHIP_REQUIRE(valid_float_dtype(d.dtype), "attention dtype must be f32 or f16");
+  AFHIP_REQUIRE(d.scale > 0.0f && d.scale < INFINITY, "scale must be positive and finite");
+  constexpr int64_t most = (int64_t)1 << 30;
+  AFHIP_REQUIRE(d.keys < most && (int64_t)d.queries * d.query_heads < most && d.query_heads <= 65536,
+                "more than 2^30 keys or queries of a sequence, or 65,536 heads");
+  AFHIP_REQUIRE((int64_t)d.batch * d.key_heads < most, "batch times heads passes 2^30");
+  WindowArgs a{};
+  window_fill(d, a);
+  int s;
+  if ((s = check_strides("q", a.sq, d.batch, d.queries, d.query_heads, d.head_dim, d.dtype, false)) ||
+      (s = check_strides("k", a.sk, d.batch, d.keys, d.key_heads, d.head_dim, d.dtype, false)) ||
+      (s = check_strides("v", a.sv, d.batch, d.keys, d.key_heads, d.head_dim, d.dtype, false)) ||
+      (s = check_strides("out", a.so, d.batch, d.queries, d.query_heads, d.head_dim, d.dtype, true)))
+    return s;
+  return AFHIP_OK;
+}
+
+void window_fill(const afhip_window_desc& d, WindowArgs& a) {
+  constexpr int most = 1 << 30;  // more than any position: sums of two stay within 32 bits
+  a.sq = head_strides(d.q, d.queries, d.query_heads, d.head_dim, d.dtype);
+  a.sk = head_strides(d.k, d.keys, d.key_heads, d.head_dim, d.dtype);
+  a.sv = head_strides(d.v, d.keys, d.key_heads, d.head_dim, d.dtype);
+  a.so = head_strides(d.out, d.queries, d.query_heads, d.head_dim, d.dtype);
+  a.batch = d.batch;
+  a.queries = d.queries;
+  a.keys = d.keys;
+  a.query_heads = d.query_heads;
+  a.key_heads = d.key_heads;
+  a.group = d.query_heads / d.key_heads;
+  a.head_dim = d.head_dim;
+  a.left = d.left >= most ? -1 : d.left;
+  a.right = d.right >= most ? -1 : d.right;
+  a.sinks = std::min(d.sinks, most);
+  a.scale = d.scale;
+  a.scale_log2 = d.scale * kWindowLog2e;
+}
+
+}  // namespace afhip
+
+using namespace afhip;
+
+extern "C" {
+
+int afhip_window_workspace_size(const afhip_window_desc* desc, size_t* bytes) {
+  if (int s = window_check(desc)) return s;
+  AFHIP_REQUIRE(bytes != nullptr, "output is NULL");
+  *bytes = partial_bytes(*desc, plan(*desc));
+  return AFHIP_OK;
+}
+
+int afhip_window_run(const afhip_window_desc* desc, const void* q, const void* k, const void* v,
+                     const int32_t* query_lengths, const int32_t* key_lengths, void* out, float* lse, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  int s;
+  if ((s = require_open()) || (s = window_check(desc))) return s;
+  const afhip_window_desc& d = *desc;
+  WindowArgs a{};
+  window_fill(d, a);
+  if ((s = check_address("q", q)) || (s = check_address("k", k)) || (s = check_address("v", v)) ||
+      (s = check_address("out", out)))
+    return s;
+  const Plan p = plan(d);
+  const size_t need = partial_bytes(d, p);
+  if (need) {
+    AFHIP_REQUIRE(workspace && workspace_bytes >= need, "workspace of %zu bytes is smaller than %zu", workspace_bytes,
+                  need);
+    if ((s = check_address("workspace", workspace))) return s;
+  }
+  a.q = (const char*)q;
+  a.k = (const char*)k;
+  a.v = (const char*)v;
+  a.out = (char*)out;
+  a.lse = lse;
+  a.query_lengths = query_lengths;
+  a.key_lengths = key_lengths;
+  a.partial = (float*)workspace;
+  a.tiles = p.tiles;
+  a.splits = p.splits;
+  hipStream_t st = (hipStream_t)stream;
+  return d.dtype == AFHIP_F16 ? launch_width<half_t>(a, p, st) : launch_width<float>(a, p, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,412 @@
+// The way back through the windowed attention (window.hip): with P = e^(s - lse), s = scale q . k, recomputed from
+// what the forward pass left, and D = sum(out * dout) of each row,
+//
+//   dv = P^T dout,  ds = P (dout V^T - D),  dq = scale ds K,  dk = scale ds^T Q.
+//
+// Two kernels, seven products in place of the least five: one holds 32 rows a wave and passes over the keys (dq), one
+// holds 32 keys a wave and passes over the rows that see them (dk and dv), all query heads of a key head among them. So
+// every gradient is summed in registers, in one order, with no atomics. Both keep the held side in registers and
+// stream the other through LDS; the probabilities and their gradients feed the next product from the registers they
+// were computed in, as in the forward pass.
+//
+// In f16, P goes into its product times 2^13 (the smallest of a row of 10^6 equal ones is then a normal number), and
+// ds, whose size nothing bounds, times a power of two that each held row (or key) lowers when a value would pass 2^15:
+// the accumulators are rescaled with it.
+#include <cmath>
+
+#include "window.h"
+
+namespace afhip {
+
+namespace {
+
+constexpr int kWaves = 4, kHeld = 32 * kWaves;
+template <typename T> constexpr int kBlock = sizeof(T) == 2 ? 64 : 32;  // keys or rows of a streamed block
+
+// A held row's power of two on ds (f16), and the accumulators it is on.
+template <typename T, int BLOCKS> struct Scaled {
+  floatx16 acc[BLOCKS];
+  float scale;
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int c = 0; c < BLOCKS; c++) acc[c] = floatx16{};
+    scale = sizeof(T) == 2 ? 0x1p126f : 1.0f;
+  }
+  // Brings ds into f16's range.
+  __device__ __forceinline__ void fit(float* ds) {
+    if constexpr (sizeof(T) == 2) {
+      float top = fabsf(ds[0]);
+#pragma unroll
+      for (int v = 1; v < 16; v++) top = fmaxf(top, fabsf(ds[v]));
+      if (__builtin_amdgcn_ballot_w64(top * scale > 0x1p15f)) {
+        const float both = fmaxf(top, __shfl_xor(top, 32));
+        // To [2^7, 2^8).
+        const float to = ldexpf(1.0f, min(126, 8 - __builtin_amdgcn_frexp_expf(both)));
+        if (both > 0.0f && to < scale) {
+          const float f = to / scale;
+#pragma unroll
+          for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) acc[c][v] *= f;
+          scale = to;
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < 16; v++) ds[v] *= scale;
+    }
+  }
+};
+
+// dq, and each row's lse and D for the other kernel. Rows as in window_rows_kernel.
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void window_dq_kernel(WindowArgs a) {
+  constexpr int BK = kBlock<T>, STEPS = DP / 16, BLOCKS = DP / 32;
+  typedef TileLoad<T, DP, BK, kWaves> Load;
+  typedef typename Eight<T>::type Frag;
+  typedef Tile<T, DP> Tl;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = a.batch * a.key_heads;
+  const int pair = blockIdx.x % heads, tile = a.tiles - 1 - blockIdx.x / heads;
+  const int b = pair / a.key_heads, kv = pair % a.key_heads;
+  const Sequence s(a, b);
+  const int rows = a.queries * a.group;
+  const int r0 = tile * kHeld, row = r0 + 32 * wave + col;
+  const int first = r0 / a.group, last = min(s.queries - 1, (r0 + kHeld - 1) / a.group);
+  const int i = row / a.group, h = kv * a.group + row % a.group;
+  const bool live = i < s.queries;
+  const int at = min(i, s.queries - 1), high = s.high(a, at), low = s.low(a, at);
+
+  Frag q[STEPS], g[STEPS];
+  float delta = 0.0f, lse = INFINITY;
+  {
+    const int64_t src = live ? i : 0;
+    const char* qp = a.q + b * a.sq.batch + src * a.sq.token + h * a.sq.head;
+    const char* gp = a.dout + b * a.sdo.batch + src * a.sdo.token + h * a.sdo.head;
+    const char* op = a.o + b * a.so.batch + src * a.so.token + h * a.so.head;
+#pragma unroll
+    for (int kk = 0; kk < STEPS; kk++) {
+      const int ch = 16 * kk + 8 * hi;
+      const bool keep = live && ch < a.head_dim;
+      q[kk] = load_eight<T>(qp, ch, keep);
+      g[kk] = load_eight<T>(gp, ch, keep);
+      const Frag o = load_eight<T>(op, ch, keep);
+#pragma unroll
+      for (int j = 0; j < 8; j++) delta += (float)o[j] * (float)g[kk][j];
+    }
+    delta += __shfl_xor(delta, 32);
+    if (live) {
+      lse = a.lse[((int64_t)b * a.query_heads + h) * a.queries + i] * kWindowLog2e;
+      if (lse == -INFINITY) lse = INFINITY;  // nothing seen: probabilities of 0
+    }
+    if (row < rows && !hi) {
+      a.rows[(int64_t)pair * rows + row] = float2{lse, delta};
+      a.limits[(int64_t)pair * rows + row] = live ? int2{high, low} : int2{0, 0};
+    }
+  }
+  Scaled<T, BLOCKS> acc;
+  acc.init();
+  if (first < s.queries) {
+    const KeyRange range(a, s, first, last, BK);
+    const int wr0 = r0 + 32 * wave;
+    const int wfirst = min(wr0 / a.group, s.queries - 1), wlast = min((wr0 + 31) / a.group, s.queries - 1);
+    const int all_low = s.low(a, wlast), all_high = s.high(a, wfirst);
+    const int any_low = s.low(a, wfirst), any_high = s.high(a, wlast);
+    const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
+    const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
+    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
+    Load load;
+    load.init(wave, lane, a.head_dim);
+    auto issue = [&](int t) {
+      const int k0 = range.block(t) * BK;
+      const uint32_t buffer = lds + (uint32_t)(t & 1) * 2 * Load::kBytes;
+      auto keep = [&](int key) { return range.keeps(key); };
+      load.issue(kb, a.sk.token, k0, buffer, wave, keep);
+      load.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, keep);
+    };
+    if (range.total > 0) issue(0);
+    for (int t = 0; t < range.total; t++) {
+      wait_vmcnt<0>();
+      block_barrier();
+      if (t + 1 < range.total) issue(t + 1);
+      const int k0 = range.block(t) * BK;
+      if (wr0 >= s.queries * a.group || k0 >= any_high || (k0 + BK <= any_low && k0 >= range.sinks)) continue;
+      const bool partial = k0 + BK > all_high || (k0 < all_low && k0 + BK > range.sinks);
+      const unsigned char* kt = smem + (t & 1) * 2 * Load::kBytes;
+      const unsigned char* vt = kt + Load::kBytes;
+#pragma unroll
+      for (int sub = 0; sub < BK; sub += 32) {
+        floatx16 x = floatx16{}, y = floatx16{};
+#pragma unroll
+        for (int kk = 0; kk < STEPS; kk++) {
+          x = mma(Tl::nat(kt, sub + col, kk, hi), q[kk], x);
+          y = mma(Tl::nat(vt, sub + col, kk, hi), g[kk], y);
+        }
+        float ds[16];
+#pragma unroll
+        for (int v = 0; v < 16; v++)
+          ds[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -lse)) * (y[v] - delta);
+        if (partial) {
+#pragma unroll
+          for (int v = 0; v < 16; v++) {
+            const int key = k0 + sub + mfma_row(v, lane);
+            if (hidden(key, low, high, range.sinks)) ds[v] = 0.0f;
+          }
+        }
+        acc.fit(ds);
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          const Frag f = pack8(ds + 8 * n, (Frag*)nullptr);
+#pragma unroll
+          for (int c = 0; c < BLOCKS; c++) acc.acc[c] = mma(Tl::tr(kt, sub + 16 * n, c, lane), f, acc.acc[c]);
+        }
+      }
+    }
+  }
+  if (row >= rows) return;
+  T* to = reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.queries + i) * a.query_heads + h) * a.head_dim;
+  const float f = a.scale / acc.scale;
+#pragma unroll
+  for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+      const int ch = 32 * c + mfma_row(v, lane);
+      if (ch < a.head_dim) to[ch] = (T)(live ? acc.acc[c][v] * f : 0.0f);
+    }
+}
+
+// dk and dv of 128 keys of a key head, over blocks of its rows.
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 128 ? 1 : 2) void window_dkv_kernel(WindowArgs a) {
+  constexpr int BR = kBlock<T>, STEPS = DP / 16, BLOCKS = DP / 32;
+  typedef Tile<T, DP> Tl;
+  typedef typename Eight<T>::type Frag;
+  constexpr int CHUNKS = Tl::kChunks, STEP = 64 / CHUNKS, COUNT = BR * CHUNKS / 64 / kWaves;
+  constexpr int TILE = BR * DP * (int)sizeof(T), STATS = 1024, BUFFER = 2 * TILE + STATS;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = a.batch * a.key_heads;
+  const int pair = blockIdx.x % heads, tile = blockIdx.x / heads;
+  const int b = pair / a.key_heads, kv = pair % a.key_heads;
+  const Sequence s(a, b);
+  const int G = a.group, rows = a.queries * G;
+  const int j0 = tile * kHeld, wj0 = j0 + 32 * wave, key = wj0 + col;
+  const bool live = key < s.keys;
+
+  Frag kf[STEPS], vf[STEPS];
+  {
+    const int64_t src = live ? key : 0;
+    const char* kp = a.k + b * a.sk.batch + src * a.sk.token + kv * a.sk.head;
+    const char* vp = a.v + b * a.sv.batch + src * a.sv.token + kv * a.sv.head;
+#pragma unroll
+    for (int kk = 0; kk < STEPS; kk++) {
+      const int ch = 16 * kk + 8 * hi;
+      kf[kk] = load_eight<T>(kp, ch, live && ch < a.head_dim);
+      vf[kk] = load_eight<T>(vp, ch, live && ch < a.head_dim);
+    }
+  }
+  Scaled<T, BLOCKS> dk;
+  floatx16 dv[BLOCKS];
+  dk.init();
+#pragma unroll
+  for (int c = 0; c < BLOCKS; c++) dv[c] = floatx16{};
+
+  // Queries that see any of keys [from, to): [first, end).
+  auto sees = [&](int from, int to, int& first, int& end) {
+    to = min(to, s.keys);
+    first = a.right < 0 ? 0 : max(0, from - a.right - s.offset);
+    end = a.left < 0 || from < a.sinks ? s.queries : min(s.queries, max(0, to + a.left - s.offset));
+    if (from >= to) end = 0;
+  };
+  int first, end, wfirst, wend;
+  sees(j0, j0 + kHeld, first, end);
+  sees(wj0, wj0 + 32, wfirst, wend);
+  if (first < end) {
+    const int begin = first * G, stop = end * G;
+    const char* qb = a.q + b * a.sq.batch + (int64_t)kv * G * a.sq.head;
+    const char* gb = a.dout + b * a.sdo.batch + (int64_t)kv * G * a.sdo.head;
+    const float per = 1.0f / (float)G;
+    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
+    const int load_row = STEP * wave + lane / CHUNKS, chunk = lane % CHUNKS;
+    const int chunks = a.head_dim * (int)sizeof(T) / 16;
+    auto issue = [&](int r0, int n) {
+      // Row r0 + r is query i0 + t / G, head t % G, with t = r + r0 % G: below 2^17, where the rounded quotient of
+      // t + 1/2 has the right whole part.
+      const int i0 = r0 / G, g0 = r0 - i0 * G;
+      const int32x4_t qr = make_rsrc(qb + (int64_t)i0 * a.sq.token, 0x7ffffff0u);
+      const int32x4_t gr = make_rsrc(gb + (int64_t)i0 * a.sdo.token, 0x7ffffff0u);
+      const uint32_t buffer = lds + (uint32_t)(n & 1) * BUFFER;
+#pragma unroll
+      for (int m = 0; m < COUNT; m++) {
+        const int r = load_row + STEP * kWaves * m, c = chunk ^ Tl::swizzle(r);
+        const int t = r + g0, i = (int)(((float)t + 0.5f) * per), g = t - i * G;
+        const bool ok = (c < chunks) & (r0 + r < stop);
+        const uint32_t q_at = (uint32_t)i * (uint32_t)a.sq.token + (uint32_t)g * (uint32_t)a.sq.head + 16u * c;
+        const uint32_t g_at = (uint32_t)i * (uint32_t)a.sdo.token + (uint32_t)g * (uint32_t)a.sdo.head + 16u * c;
+        dma16(qr, buffer + 1024 * (wave + kWaves * m), ok ? q_at : kOutOfRange);
+        dma16(gr, buffer + TILE + 1024 * (wave + kWaves * m), ok ? g_at : kOutOfRange);
+      }
+      // The rows' statistics, 8 bytes each, 32 rows an instruction: lse and D, and the keys they see. Past the last
+      // row zeros, whose rows of dout are zeros too.
+      const int part = 32 * (wave & 1), left = stop - r0 - part;
+      if (part < BR) {
+        const int64_t at = (int64_t)pair * rows + r0 + part;
+        const int32x4_t sr = make_rsrc(wave < 2 ? (const void*)(a.rows + at) : (const void*)(a.limits + at),
+                                       8u * (uint32_t)max(0, min(32, left)));
+        dma4(sr, buffer + 2 * TILE + 8 * (wave < 2 ? 0 : BR) + 8 * part, 4u * lane);
+      }
+    };
+    issue(begin, 0);
+    int n = 0;
+    for (int r0 = begin; r0 < stop; r0 += BR, n++) {
+      wait_vmcnt<0>();
+      block_barrier();
+      if (r0 + BR < stop) issue(r0 + BR, n + 1);
+      const int bfirst = r0 / G, blast = min(end - 1, (r0 + BR - 1) / G);
+      if (blast < wfirst || bfirst >= wend) continue;
+      const bool partial = wj0 + 32 > s.high(a, bfirst) || (wj0 < s.low(a, blast) && wj0 + 32 > a.sinks);
+      const unsigned char* qt = smem + (n & 1) * BUFFER;
+      const unsigned char* gt = qt + TILE;
+      const float2* stats = reinterpret_cast<const float2*>(gt + TILE);
+#pragma unroll
+      for (int sub = 0; sub < BR; sub += 32) {
+        floatx16 x = floatx16{}, y = floatx16{};
+#pragma unroll
+        for (int kk = 0; kk < STEPS; kk++) {
+          x = mma(Tl::nat(qt, sub + col, kk, hi), kf[kk], x);
+          y = mma(Tl::nat(gt, sub + col, kk, hi), vf[kk], y);
+        }
+        float p[16], ds[16];
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+          const float2 st = stats[sub + mfma_row(v, lane)];
+          p[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -st.x));
+          ds[v] = p[v] * (y[v] - st.y);
+        }
+        if (partial) {
+          const int2* limits = reinterpret_cast<const int2*>(stats + BR);
+#pragma unroll
+          for (int v = 0; v < 16; v++) {
+            const int2 lim = limits[sub + mfma_row(v, lane)];
+            if (hidden(key, lim.y, lim.x, a.sinks)) p[v] = ds[v] = 0.0f;
+          }
+        }
+        dk.fit(ds);
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int v = 0; v < 16; v++) p[v] *= 0x1p13f;
+        }
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+          const Frag pf = pack8(p + 8 * m, (Frag*)nullptr), df = pack8(ds + 8 * m, (Frag*)nullptr);
+#pragma unroll
+          for (int c = 0; c < BLOCKS; c++) {
+            dv[c] = mma(Tl::tr(gt, sub + 16 * m, c, lane), pf, dv[c]);
+            dk.acc[c] = mma(Tl::tr(qt, sub + 16 * m, c, lane), df, dk.acc[c]);
+          }
+        }
+      }
+    }
+  }
+  if (key >= a.keys) return;
+  const int64_t at = (((int64_t)b * a.keys + key) * a.key_heads + kv) * a.head_dim;
+  T *tk = reinterpret_cast<T*>(a.dk) + at, *tv = reinterpret_cast<T*>(a.dv) + at;
+  const float fk = a.scale / dk.scale, fv = sizeof(T) == 2 ? 0x1p-13f : 1.0f;
+#pragma unroll
+  for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+      const int ch = 32 * c + mfma_row(v, lane);
+      if (ch >= a.head_dim) continue;
+      tk[ch] = (T)(live ? dk.acc[c][v] * fk : 0.0f);
+      tv[ch] = (T)(live ? dv[c][v] * fv : 0.0f);
+    }
+}
+
+template <typename T, int DP> int launch_backward(WindowArgs& a, hipStream_t st) {
+  int s;
+  const int64_t heads = (int64_t)a.batch * a.key_heads, rows = (int64_t)a.queries * a.group;
+  a.tiles = (int)ceil_div(rows, kHeld);
+  AFHIP_REQUIRE(heads * a.tiles < ((int64_t)1 << 31) && heads * ceil_div(a.keys, kHeld) < ((int64_t)1 << 31),
+                "attention grid too large");
+  constexpr size_t lds_q = 4 * kBlock<T> * DP * sizeof(T), lds_kv = 2 * (2 * kBlock<T> * DP * sizeof(T) + 1024);
+  auto kq = window_dq_kernel<T, DP>;
+  if ((s = allow_lds((const void*)kq, lds_q))) return s;
+  if ((s = launch("window.dq", kq, dim3((unsigned)(heads * a.tiles)), dim3(64 * kWaves), lds_q, st, a))) return s;
+  auto kkv = window_dkv_kernel<T, DP>;
+  if ((s = allow_lds((const void*)kkv, lds_kv))) return s;
+  return launch("window.dkv", kkv, dim3((unsigned)(heads * ceil_div(a.keys, kHeld))), dim3(64 * kWaves), lds_kv, st,
+                a);
+}
+
+template <typename T> int launch_width(WindowArgs& a, hipStream_t st) {
+  if (a.head_dim <= 32) return launch_backward<T, 32>(a, st);
+  if (a.head_dim <= 64) return launch_backward<T, 64>(a, st);
+  return launch_backward<T, 128>(a, st);
+}
+
+size_t row_bytes(const afhip_window_desc& d) {
+  return (size_t)round_up((int64_t)d.batch * d.queries * d.query_heads * 8, 256);
+}
+
+}  // namespace
+
+}  // namespace afhip
+
+using namespace afhip;
+
+extern "C" {
+
+int afhip_window_backward_workspace_size(const afhip_window_desc* desc, size_t* bytes) {
+  if (int s = window_check(desc)) return s;
+  AFHIP_REQUIRE(bytes != nullptr, "output is NULL");
+  *bytes = 2 * row_bytes(*desc);
+  return AFHIP_OK;
+}
+
+int afhip_window_backward(const afhip_window_desc* desc, const void* q, const void* k, const void* v, const void* out,
+                          const float* lse, const void* dout, const afhip_strides* dout_strides,
+                          const int32_t* query_lengths, const int32_t* key_lengths, void* dq, void* dk, void* dv,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+  int s;
+  size_t need = 0;
+  if ((s = require_open()) || (s = afhip_window_backward_workspace_size(desc, &need))) return s;
+  const afhip_window_desc& d = *desc;
+  WindowArgs a{};
+  window_fill(d, a);
+  AFHIP_REQUIRE(dout_strides != nullptr, "the strides of dout are NULL");
+  a.sdo = head_strides(*dout_strides, d.queries, d.query_heads, d.head_dim, d.dtype);
+  if ((s = check_strides("dout", a.sdo, d.batch, d.queries, d.query_heads, d.head_dim, d.dtype, false)) ||
+      (s = check_address("q", q)) || (s = check_address("k", k)) || (s = check_address("v", v)) ||
+      (s = check_address("out", out)) || (s = check_address("dout", dout)) || (s = check_address("dq", dq)) ||
+      (s = check_address("dk", dk)) || (s = check_address("dv", dv)))
+    return s;
+  // Rows of a block lie within a buffer's 2 GiB: 65 queries, and the group's heads beside them.
+  for (const HeadStrides* x : {&a.sq, &a.sdo})
+    AFHIP_REQUIRE(65 * x->token + (int64_t)a.group * x->head < ((int64_t)1 << 31),
+                  "the heads of a group are more than 2 GiB apart");
+  AFHIP_REQUIRE(lse != nullptr, "lse is NULL");
+  AFHIP_REQUIRE(workspace && workspace_bytes >= need, "workspace of %zu bytes is smaller than %zu", workspace_bytes,
+                need);
+  if ((s = check_address("workspace", workspace))) return s;
+  a.q = (const char*)q;
+  a.k = (const char*)k;
+  a.v = (const char*)v;
+  a.o = (const char*)out;
+  a.lse = const_cast<float*>(lse);
+  a.dout = (const char*)dout;
+  a.query_lengths = query_lengths;
+  a.key_lengths = key_lengths;
+  a.dq = (char*)dq;
+  a.dk = (char*)dk;
+  a.dv = (char*)dv;
+  a.rows = (float2*)workspace;
+  a.limits = (int2*)((char*)workspace + row_bytes(d));
+  hipStream_t st = (hipStream_t)stream;
+  return d.dtype == AFHIP_F16 ? launch_width<half_t>(a, st) : launch_width<float>(a, st);
+}
+
+}  // extern "C"

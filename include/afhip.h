@@ -466,6 +466,108 @@ AFHIP_API int afhip_attention_run(const afhip_attention_desc* desc, const void* 
                         size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------- */
+/* Heads of one sequence: norm, rotation, cache, windowed attention        */
+/* ---------------------------------------------------------------------- */
+
+/* Where an element of a tensor [batch][tokens][heads][channels] lies, in
+ * elements; channels are contiguous. token 0: packed, in that order. A batch
+ * or head stride of 0 repeats one entry (inputs only). Strides that are used
+ * are multiples of 16 bytes, and so are all tensors' addresses. No counterpart
+ * in the reference (its tensors are packed) here and in the rest of this section. */
+typedef struct afhip_strides {
+  int64_t batch, token, head;
+} afhip_strides;
+
+/* Which channels turn together, of the first rotary_dim = 2 n: (j, j + n) or
+ * (2 j, 2 j + 1). */
+#define AFHIP_ROTARY_HALF 0
+#define AFHIP_ROTARY_INTERLEAVED 1
+
+#define AFHIP_HEAD_NORM_NONE 0
+#define AFHIP_HEAD_NORM_RMS 1   /* x / sqrt(mean(x^2) + epsilon) * scale */
+#define AFHIP_HEAD_NORM_LAYER 2 /* (x - mean) / sqrt(variance + epsilon) * scale + offset */
+
+/* The norm of each query and key head and the rotation by its position, in
+ * one pass; the keys, and the values beside them, go into a cache where
+ * capacity is positive. */
+typedef struct afhip_rotary_desc {
+  int32_t batch, tokens;
+  int32_t query_heads, key_heads;
+  int32_t head_dim;   /* a multiple of 8, at most 128 */
+  int32_t rotary_dim; /* a multiple of 8, at most head_dim; 0 turns nothing */
+  int32_t layout;     /* AFHIP_ROTARY_* */
+  int32_t norm;       /* AFHIP_HEAD_NORM_* */
+  int32_t dtype;      /* of every tensor with channels: AFHIP_F32 | AFHIP_F16 */
+  int32_t capacity;   /* tokens a sequence's cache (k_out, v_out) holds; 0: k_out is [batch][tokens] */
+  float epsilon;
+  float rotation_scale;                          /* a factor on the channels that turn */
+  afhip_strides q, k, v, q_out, k_out, v_out;
+} afhip_rotary_desc;
+
+/* past, lengths: i32 [batch] or NULL: tokens that a sequence has behind it
+ * (0), and how many of `tokens` it has (all). positions: i32 [batch][tokens]
+ * or NULL (past + i). frequencies: f64 [rotary_dim / 2], the angle of one
+ * position. Angles are taken in 64 bits. scales and offsets: f32 [head_dim] as
+ * the norm has them. q_out may be q, and k_out k where there is no cache.
+ * A token past its sequence's length gives zeros in q_out (and in a k_out
+ * without a cache) and writes nothing into a cache; a token i goes to the
+ * cache's row past + i, and is not written where that is outside [0, capacity).
+ * v and v_out may be NULL together; without a cache they must be. */
+AFHIP_API int afhip_rotary_run(const afhip_rotary_desc* desc, const void* q, const void* k, const void* v,
+                               const int32_t* past, const int32_t* lengths, const int32_t* positions,
+                               const double* frequencies, const float* query_scale, const float* query_offset,
+                               const float* key_scale, const float* key_offset, void* q_out, void* k_out,
+                               void* v_out, void* stream);
+/* The way back: dq, dk from the gradients of q_out and k_out, and those of the
+ * norm's vectors (f32 [head_dim]; as the norm has them). capacity must be 0;
+ * the descriptor's q and k are the strides of q and k, q_out and k_out those
+ * of dq_out, dk_out, and dq, dk are packed. Every row of dq and dk is written,
+ * zeros past the lengths. Sums in a fixed order. */
+AFHIP_API int afhip_rotary_backward_workspace_size(const afhip_rotary_desc* desc, size_t* bytes);
+AFHIP_API int afhip_rotary_backward(const afhip_rotary_desc* desc, const void* q, const void* k,
+                                    const int32_t* past, const int32_t* lengths, const int32_t* positions,
+                                    const double* frequencies, const float* query_scale, const float* key_scale,
+                                    const void* dq_out, const void* dk_out, void* dq, void* dk,
+                                    float* dquery_scale, float* dquery_offset, float* dkey_scale,
+                                    float* dkey_offset, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention over a window of keys and the first few ("sinks"). Queries are the
+ * last of their sequence: query i has position p = key_length - query_length +
+ * i, and sees key j where j < key_length, j <= p + right, and j >= p - left or
+ * j < sinks. Query head h reads key head h / (query_heads / key_heads). */
+typedef struct afhip_window_desc {
+  int32_t batch, queries, keys; /* keys: rows of k and v, a cache's capacity for instance */
+  int32_t query_heads, key_heads;
+  int32_t head_dim;    /* a multiple of 8, at most 128 */
+  int32_t left, right; /* -1: no end on that side */
+  int32_t sinks;
+  int32_t dtype;       /* AFHIP_F32 | AFHIP_F16; products and sums in f32 */
+  float scale;         /* on q . k, positive */
+  afhip_strides q, k, v, out;
+} afhip_window_desc;
+
+/* query_lengths, key_lengths: i32 [batch] or NULL (all); values outside
+ * [0, queries] and [0, keys] are taken as the nearer end. out [batch][queries]
+ * [query_heads][head_dim]; lse, the natural logarithm of each row's sum of
+ * exponentials, f32 [batch][query_heads][queries], or NULL. A row that sees
+ * nothing, or past its sequence's length, gives zeros and an lse of -infinity;
+ * keys past the length are never read. */
+AFHIP_API int afhip_window_workspace_size(const afhip_window_desc* desc, size_t* bytes);
+AFHIP_API int afhip_window_run(const afhip_window_desc* desc, const void* q, const void* k, const void* v,
+                               const int32_t* query_lengths, const int32_t* key_lengths, void* out, float* lse,
+                               void* workspace, size_t workspace_bytes, void* stream);
+/* The gradients of q, k and v (packed; k's and v's summed over the heads that
+ * read them) from what the forward pass left and the gradient of out. The
+ * descriptor's out are out's strides; dout's are given. Every row is written,
+ * zeros past the lengths. Sums in a fixed order. */
+AFHIP_API int afhip_window_backward_workspace_size(const afhip_window_desc* desc, size_t* bytes);
+AFHIP_API int afhip_window_backward(const afhip_window_desc* desc, const void* q, const void* k, const void* v,
+                                    const void* out, const float* lse, const void* dout,
+                                    const afhip_strides* dout_strides, const int32_t* query_lengths,
+                                    const int32_t* key_lengths, void* dq, void* dk, void* dv, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------- */
 /* Execution layer                                                         */
 /* ---------------------------------------------------------------------- */
 
