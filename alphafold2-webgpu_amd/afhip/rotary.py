@@ -13,8 +13,8 @@ import math
 import numpy as np
 
 from . import _lib
-from .device import device, empty_bytes, open_device
-from .heads import FORMS, address, check_device, check_heads, check_ints, form, strides
+from .device import device, open_device
+from .heads import FORMS, address, check_device, check_heads, check_ints, current_stream, form, packed_like, strides
 
 _DT = {"f32": _lib.F32, "f16": _lib.F16}
 _LAYOUTS = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
@@ -87,7 +87,8 @@ class HeadRotary:
             raise _lib.RangeError(f"frequencies has {f.numel()} values; expected {self.rotary_dim // 2}")
         self.frequencies = f.to(device()).contiguous()
         self._torch_dtype = torch.float32 if dtype == "f32" else torch.float16
-        self._device = device().index
+        self._torch_device = device()
+        self._device = self._torch_device.index
         self._forms = {}
         self.query_scale = self.key_scale = self.query_offset = self.key_offset = None
 
@@ -163,14 +164,14 @@ class HeadRotary:
                 self._forms.clear()
             self._forms[key] = desc
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = packed_like(q)
         if k_cache is None and k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            k_out = packed_like(k)
         _lib.call("afhip_rotary_run", desc, q.data_ptr(), k.data_ptr(), address(v), address(past), address(lengths),
                   address(positions), self.frequencies.data_ptr(), address(self.query_scale),
                   address(self.query_offset), address(self.key_scale), address(self.key_offset), q_out.data_ptr(),
                   (k_out if k_cache is None else k_cache).data_ptr(), address(v_cache),
-                  torch.cuda.current_stream().cuda_stream)
+                  current_stream(self._device))
         return (q_out, k_out) if k_cache is None else (q_out, k_cache, v_cache)
 
     def _form(self, q, k, v, past, lengths, positions, q_out, k_out, k_cache, v_cache):
@@ -222,8 +223,7 @@ class HeadRotary:
                 self._forms.clear()
             found = self._forms[key] = (ctypes.pointer(desc), size.value)
         desc, bytes_ = found
-        out = {"dq": torch.empty(q.shape, dtype=q.dtype, device=q.device),
-               "dk": torch.empty(k.shape, dtype=k.dtype, device=k.device)}
+        out = {"dq": packed_like(q), "dk": packed_like(k)}
         if self.norm is not None:
             out["dquery_scale"] = torch.empty_like(self.query_scale)
             out["dkey_scale"] = torch.empty_like(self.key_scale)
@@ -231,11 +231,11 @@ class HeadRotary:
                 out["dquery_offset"] = torch.empty_like(self.query_scale)
                 out["dkey_offset"] = torch.empty_like(self.key_scale)
         # From the caching allocator at each call: calls on several streams, and captured ones, share nothing.
-        workspace = empty_bytes(bytes_)
+        workspace = torch.empty(max(bytes_, 1), dtype=torch.uint8, device=self._torch_device)
         _lib.call("afhip_rotary_backward", desc, q.data_ptr(), k.data_ptr(), address(past), address(lengths),
                   address(positions), self.frequencies.data_ptr(), address(self.query_scale),
                   address(self.key_scale), dq_out.data_ptr(), dk_out.data_ptr(), out["dq"].data_ptr(),
                   out["dk"].data_ptr(), address(out.get("dquery_scale")), address(out.get("dquery_offset")),
                   address(out.get("dkey_scale")), address(out.get("dkey_offset")), workspace.data_ptr(), bytes_,
-                  torch.cuda.current_stream().cuda_stream)
+                  current_stream(self._device))
         return out

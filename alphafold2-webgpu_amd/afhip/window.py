@@ -13,8 +13,8 @@ import ctypes
 import math
 
 from . import _lib
-from .device import device, empty_bytes, open_device
-from .heads import FORMS, address, check_device, check_heads, check_ints, form, strides
+from .device import device, open_device
+from .heads import FORMS, address, check_device, check_heads, check_ints, current_stream, form, packed_like, strides
 
 _DT = {"f32": _lib.F32, "f16": _lib.F16}
 
@@ -42,7 +42,8 @@ class WindowAttention:
         probe = self._desc(1, 1, 1)  # refuses what no call can have
         _lib.call("afhip_window_workspace_size", ctypes.byref(probe), ctypes.byref(ctypes.c_size_t()))
         self._torch_dtype = torch.float32 if dtype == "f32" else torch.float16
-        self._device = device().index
+        self._torch_device = device()
+        self._device = self._torch_device.index
         self._forms = {}
 
     def _desc(self, batch: int, queries: int, keys: int, **tensors) -> _lib.WindowDesc:
@@ -91,13 +92,13 @@ class WindowAttention:
             found = self._remember(key, (ctypes.pointer(desc), size.value, (batch, self.query_heads, queries)))
         desc, bytes_, rows = found
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(rows, dtype=torch.float32, device=q.device) if return_lse else None
+            out = packed_like(q)
+        lse = torch.empty(rows, dtype=torch.float32, device=self._torch_device) if return_lse else None
         # From the caching allocator at each call: calls on several streams, and captured ones, share nothing.
-        workspace = empty_bytes(bytes_) if bytes_ else None
+        workspace = torch.empty(bytes_, dtype=torch.uint8, device=self._torch_device) if bytes_ else None
         _lib.call("afhip_window_run", desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), address(query_lengths),
                   address(key_lengths), out.data_ptr(), address(lse), address(workspace), bytes_,
-                  torch.cuda.current_stream().cuda_stream)
+                  current_stream(self._device))
         return (out, lse) if return_lse else out
 
     def backward(self, q, k, v, out, lse, dout, *, query_lengths=None, key_lengths=None) -> tuple:
@@ -124,10 +125,10 @@ class WindowAttention:
             _lib.call("afhip_window_backward_workspace_size", ctypes.byref(desc), ctypes.byref(size))
             found = self._remember(key, (ctypes.pointer(desc), ctypes.pointer(strides(dout)), size.value))
         desc, dout_strides, bytes_ = found
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-        workspace = empty_bytes(bytes_)
+        dq, dk, dv = packed_like(q), packed_like(k), packed_like(v)
+        workspace = torch.empty(max(bytes_, 1), dtype=torch.uint8, device=self._torch_device)
         _lib.call("afhip_window_backward", desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                   lse.data_ptr(), dout.data_ptr(), dout_strides, address(query_lengths), address(key_lengths),
                   dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(), bytes_,
-                  torch.cuda.current_stream().cuda_stream)
+                  current_stream(self._device))
         return dq, dk, dv

@@ -16,7 +16,8 @@ struct WindowArgs {
   char* out;
   float* lse;
   const int32_t *query_lengths, *key_lengths;
-  float* partial;  // split keys: [row][split] of head_dim sums, the reference point, the total
+  // Split keys: [row][split] of head_dim sums, the reference point, the total. The way back: [tile][chunk] of dk and dv.
+  float* partial;
   HeadStrides sq, sk, sv, so;
   int batch, queries, keys, query_heads, key_heads, group, head_dim;
   int left, right, sinks;
@@ -29,6 +30,7 @@ struct WindowArgs {
   // [batch][key head][row]: the row's lse in base 2 and the sum of out * dout; the keys it sees, below and from.
   float2* rows;
   int2* limits;
+  int chunks, chunk_rows;  // dk and dv: the most chunks of rows that a tile of keys has, and the rows of one
 };
 
 typedef float floatx8 __attribute__((ext_vector_type(8)));
@@ -112,8 +114,8 @@ template <typename T, int DP, int ROWS, int WAVES> struct TileLoad {
     chunks = head_dim * (int)sizeof(T) / 16;
   }
 
-  // Rows row0 .. of the tensor at `base`, those that keep(row) holds for; zeros for the others. At most 64 rows of
-  // token strides up to 2^24 bytes: offsets stay below 2^30.
+  // Rows row0 .. of the tensor at `base`, those that keep(row) holds for; zeros for the others. At most 127 rows
+  // of token strides up to 2^24 bytes after the first: offsets stay below 2^31.
   template <typename Keep>
   __device__ __forceinline__ void issue(const char* base, int64_t token, int row0, uint32_t lds, int wave,
                                         Keep keep) const {
@@ -144,6 +146,14 @@ __device__ __forceinline__ half8 pack8(const float* x, half8*) {
 }
 __device__ __forceinline__ floatx8 pack8(const float* x, floatx8*) {
   return floatx8{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+}
+
+// Writes four channels.
+__device__ __forceinline__ void put4(half_t* p, float a, float b, float c, float d) {
+  *reinterpret_cast<half4*>(p) = half4{(half_t)a, (half_t)b, (half_t)c, (half_t)d};
+}
+__device__ __forceinline__ void put4(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<floatx4*>(p) = floatx4{a, b, c, d};
 }
 
 // One sequence: its numbers of queries and keys, and where its queries start.

@@ -115,14 +115,6 @@ template <typename T, int DP> struct Rows {
   }
 };
 
-// Writes four channels.
-__device__ __forceinline__ void put4(half_t* p, float a, float b, float c, float d) {
-  *reinterpret_cast<half4*>(p) = half4{(half_t)a, (half_t)b, (half_t)c, (half_t)d};
-}
-__device__ __forceinline__ void put4(float* p, float a, float b, float c, float d) {
-  *reinterpret_cast<floatx4*>(p) = floatx4{a, b, c, d};
-}
-
 // The natural logarithm of a row's sum, from its reference point and total (both in base 2).
 template <typename T> __device__ __forceinline__ float row_lse(float m, float l) {
   return l == 0.0f ? -INFINITY : (m - kLift<T> + log2f(l)) * kWindowLn2;
@@ -344,16 +336,25 @@ template <typename T> __global__ __launch_bounds__(256) void window_join_kernel(
   float m = mine;
 #pragma unroll
   for (int step = 1; step < 64; step *= 2) m = fmaxf(m, __shfl_xor(m, step));
-  const float f = mine == m ? 1.0f : __builtin_amdgcn_exp2f(mine - m);
+  const float f = lane >= a.splits ? 0.0f : mine == m ? 1.0f : __builtin_amdgcn_exp2f(mine - m);
   float total = lane < a.splits ? f * at[1] : 0.0f;
 #pragma unroll
   for (int step = 1; step < 64; step *= 2) total += __shfl_xor(total, step);
+  // Eight parts' loads at once; past the last part its own again, with a weight of 0.
   float o[2] = {0.0f, 0.0f};
-  for (int k = 0; k < a.splits; k++) {
-    const float w = __shfl(f, k);
+  for (int k0 = 0; k0 < a.splits; k0 += 8) {
+    float x[8][2];
 #pragma unroll
-    for (int j = 0; j < 2; j++)
-      if (lane + 64 * j < a.head_dim) o[j] += w * from[(int64_t)k * (a.head_dim + 2) + lane + 64 * j];
+    for (int k = 0; k < 8; k++)
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+        x[k][j] = from[(int64_t)min(k0 + k, a.splits - 1) * (a.head_dim + 2) + min(lane + 64 * j, a.head_dim - 1)];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float w = __shfl(f, k0 + k);
+#pragma unroll
+      for (int j = 0; j < 2; j++) o[j] += w * x[k][j];
+    }
   }
   const bool live = i < s.queries && total != 0.0f;
   T* to = reinterpret_cast<T*>(a.out + b * a.so.batch + i * a.so.token + h * a.so.head);

@@ -12,6 +12,7 @@
 // In f16, P goes into its product times 2^13 (the smallest of a row of 10^6 equal ones is then a normal number), and
 // ds, whose size nothing bounds, times a power of two that each held row (or key) lowers when a value would pass 2^15:
 // the accumulators are rescaled with it.
+#include <algorithm>
 #include <cmath>
 
 #include "window.h"
@@ -177,26 +178,71 @@ __global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void win
     }
 }
 
-// dk and dv of 128 keys of a key head, over blocks of its rows.
+// dk and dv of a tile of keys of a key head, over blocks of its rows: KEYS groups of 32 keys, each with ROWS waves that
+// take 32 rows of a block in turn and meet in LDS at the end. Each wave reads every row of its part four times from
+// LDS (for two products as it lies and for two transposed), which takes as long as its MFMAs: eight waves a CU let the
+// one hide behind the other.
+//
+// Tiles differ in how many rows see them (those of the sinks: all), and few sequences have few tiles: the rows are cut
+// into chunks, and a tile of several leaves partial sums, joined by window_dkv_join_kernel.
+template <typename T, int DP> struct KeyTile {
+  static constexpr int kKeyGroups = DP * sizeof(T) > 256 ? 2 : 4, kRowGroups = 2, kThreads = 64 * kKeyGroups * kRowGroups;
+  static constexpr int kKeys = 32 * kKeyGroups, kRows = 32 * kRowGroups;
+  static constexpr int kStats = 16 * kRows;  // the rows' statistics and limits
+  static constexpr int kTileBytes = kRows * DP * (int)sizeof(T), kBuffer = 2 * kTileBytes + kStats;
+  // Whether V is read from LDS at each block, a quarter more of LDS reads, where K, V and the sums would leave no
+  // registers to read fragments ahead of their MFMAs.
+  static constexpr bool kShareV = DP == 128 && sizeof(T) == 2;
+  static constexpr int kVBytes = kShareV ? kKeys * DP * (int)sizeof(T) : 0, kLds = 2 * kBuffer + kVBytes;
+  static_assert(kLds >= kKeyGroups * DP * 128, "a group's accumulators of one gradient fit");
+};
+
+// Rows that see any key of a tile, and its chunks of them.
+struct TileRows {
+  int begin, stop, chunks;
+  __device__ __forceinline__ TileRows(const WindowArgs& a, const Sequence& s, int from, int to) {
+    int first, end;
+    queries(a, s, from, to, first, end);
+    begin = first * a.group;
+    stop = max(begin, end * a.group);
+    chunks = (stop - begin + a.chunk_rows - 1) / a.chunk_rows;
+  }
+  // Queries [first, end) that see any of keys [from, to).
+  static __device__ __forceinline__ void queries(const WindowArgs& a, const Sequence& s, int from, int to, int& first,
+                                                 int& end) {
+    to = min(to, s.keys);
+    first = a.right < 0 ? 0 : max(0, from - a.right - s.offset);
+    end = a.left < 0 || from < a.sinks ? s.queries : min(s.queries, max(0, to + a.left - s.offset));
+    if (from >= to) end = 0;
+  }
+};
+
+template <typename T, int DP> constexpr int kKeyTileThreads = KeyTile<T, DP>::kThreads;
+
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 128 ? 1 : 2) void window_dkv_kernel(WindowArgs a) {
-  constexpr int BR = kBlock<T>, STEPS = DP / 16, BLOCKS = DP / 32;
+__global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(WindowArgs a) {
+  typedef KeyTile<T, DP> KT;
   typedef Tile<T, DP> Tl;
   typedef typename Eight<T>::type Frag;
-  constexpr int CHUNKS = Tl::kChunks, STEP = 64 / CHUNKS, COUNT = BR * CHUNKS / 64 / kWaves;
-  constexpr int TILE = BR * DP * (int)sizeof(T), STATS = 1024, BUFFER = 2 * TILE + STATS;
+  constexpr int BR = KT::kRows, STEPS = DP / 16, BLOCKS = DP / 32, WAVES = KT::kThreads / 64;
+  constexpr int CHUNKS = Tl::kChunks, STEP = 64 / CHUNKS, COUNT = BR * CHUNKS / 64;
+  constexpr int TILE = KT::kTileBytes;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = wave % KT::kKeyGroups, rg = wave / KT::kKeyGroups;
   const int heads = a.batch * a.key_heads;
-  const int pair = blockIdx.x % heads, tile = blockIdx.x / heads;
+  const int pair = blockIdx.x % heads, rest = blockIdx.x / heads, tile = rest / a.chunks, chunk = rest % a.chunks;
   const int b = pair / a.key_heads, kv = pair % a.key_heads;
   const Sequence s(a, b);
   const int G = a.group, rows = a.queries * G;
-  const int j0 = tile * kHeld, wj0 = j0 + 32 * wave, key = wj0 + col;
+  const int j0 = tile * KT::kKeys, wj0 = j0 + 32 * kg, key = wj0 + col;
   const bool live = key < s.keys;
+  const TileRows range(a, s, j0, j0 + KT::kKeys);
+  if (chunk > 0 && chunk >= range.chunks) return;
+  const int begin = range.begin + chunk * a.chunk_rows, stop = min(range.stop, begin + a.chunk_rows);
 
-  Frag kf[STEPS], vf[STEPS];
+  Frag kf[STEPS], vf[KT::kShareV ? 1 : STEPS];
   {
     const int64_t src = live ? key : 0;
     const char* kp = a.k + b * a.sk.batch + src * a.sk.token + kv * a.sk.head;
@@ -205,32 +251,23 @@ __global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 128 ? 1 : 2) void win
     for (int kk = 0; kk < STEPS; kk++) {
       const int ch = 16 * kk + 8 * hi;
       kf[kk] = load_eight<T>(kp, ch, live && ch < a.head_dim);
-      vf[kk] = load_eight<T>(vp, ch, live && ch < a.head_dim);
+      if constexpr (!KT::kShareV) vf[kk] = load_eight<T>(vp, ch, live && ch < a.head_dim);
     }
   }
+  const unsigned char* vt = smem + 2 * KT::kBuffer;
   Scaled<T, BLOCKS> dk;
   floatx16 dv[BLOCKS];
   dk.init();
 #pragma unroll
   for (int c = 0; c < BLOCKS; c++) dv[c] = floatx16{};
 
-  // Queries that see any of keys [from, to): [first, end).
-  auto sees = [&](int from, int to, int& first, int& end) {
-    to = min(to, s.keys);
-    first = a.right < 0 ? 0 : max(0, from - a.right - s.offset);
-    end = a.left < 0 || from < a.sinks ? s.queries : min(s.queries, max(0, to + a.left - s.offset));
-    if (from >= to) end = 0;
-  };
-  int first, end, wfirst, wend;
-  sees(j0, j0 + kHeld, first, end);
-  sees(wj0, wj0 + 32, wfirst, wend);
-  if (first < end) {
-    const int begin = first * G, stop = end * G;
+  if (begin < stop) {
+    int wfirst, wend;
+    TileRows::queries(a, s, wj0, wj0 + 32, wfirst, wend);
     const char* qb = a.q + b * a.sq.batch + (int64_t)kv * G * a.sq.head;
     const char* gb = a.dout + b * a.sdo.batch + (int64_t)kv * G * a.sdo.head;
     const float per = 1.0f / (float)G;
     const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
-    const int load_row = STEP * wave + lane / CHUNKS, chunk = lane % CHUNKS;
     const int chunks = a.head_dim * (int)sizeof(T) / 16;
     auto issue = [&](int r0, int n) {
       // Row r0 + r is query i0 + t / G, head t % G, with t = r + r0 % G: below 2^17, where the rounded quotient of
@@ -238,114 +275,236 @@ __global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 128 ? 1 : 2) void win
       const int i0 = r0 / G, g0 = r0 - i0 * G;
       const int32x4_t qr = make_rsrc(qb + (int64_t)i0 * a.sq.token, 0x7ffffff0u);
       const int32x4_t gr = make_rsrc(gb + (int64_t)i0 * a.sdo.token, 0x7ffffff0u);
-      const uint32_t buffer = lds + (uint32_t)(n & 1) * BUFFER;
-#pragma unroll
-      for (int m = 0; m < COUNT; m++) {
-        const int r = load_row + STEP * kWaves * m, c = chunk ^ Tl::swizzle(r);
+      const uint32_t buffer = lds + (uint32_t)(n & 1) * KT::kBuffer;
+      for (int m = wave; m < COUNT; m += WAVES) {
+        const int r = STEP * m + lane / CHUNKS, c = (lane % CHUNKS) ^ Tl::swizzle(r);
         const int t = r + g0, i = (int)(((float)t + 0.5f) * per), g = t - i * G;
         const bool ok = (c < chunks) & (r0 + r < stop);
         const uint32_t q_at = (uint32_t)i * (uint32_t)a.sq.token + (uint32_t)g * (uint32_t)a.sq.head + 16u * c;
         const uint32_t g_at = (uint32_t)i * (uint32_t)a.sdo.token + (uint32_t)g * (uint32_t)a.sdo.head + 16u * c;
-        dma16(qr, buffer + 1024 * (wave + kWaves * m), ok ? q_at : kOutOfRange);
-        dma16(gr, buffer + TILE + 1024 * (wave + kWaves * m), ok ? g_at : kOutOfRange);
+        dma16(qr, buffer + 1024 * m, ok ? q_at : kOutOfRange);
+        dma16(gr, buffer + TILE + 1024 * m, ok ? g_at : kOutOfRange);
       }
       // The rows' statistics, 8 bytes each, 32 rows an instruction: lse and D, and the keys they see. Past the last
       // row zeros, whose rows of dout are zeros too.
-      const int part = 32 * (wave & 1), left = stop - r0 - part;
-      if (part < BR) {
+      if (wave < 2 * KT::kRowGroups) {
+        const int part = 32 * (wave >> 1);
         const int64_t at = (int64_t)pair * rows + r0 + part;
-        const int32x4_t sr = make_rsrc(wave < 2 ? (const void*)(a.rows + at) : (const void*)(a.limits + at),
-                                       8u * (uint32_t)max(0, min(32, left)));
-        dma4(sr, buffer + 2 * TILE + 8 * (wave < 2 ? 0 : BR) + 8 * part, 4u * lane);
+        const int32x4_t sr = make_rsrc(wave & 1 ? (const void*)(a.limits + at) : (const void*)(a.rows + at),
+                                       8u * (uint32_t)max(0, min(32, stop - r0 - part)));
+        dma4(sr, buffer + 2 * TILE + 8 * (wave & 1 ? BR : 0) + 8 * part, 4u * lane);
       }
     };
+    if constexpr (KT::kShareV) {
+      TileLoad<T, DP, KT::kKeys, WAVES> load;
+      load.init(wave, lane, a.head_dim);
+      load.issue(a.v + b * a.sv.batch + kv * a.sv.head, a.sv.token, j0, lds + 2 * KT::kBuffer, wave,
+                 [&](int key) { return key < s.keys; });
+    }
     issue(begin, 0);
     int n = 0;
     for (int r0 = begin; r0 < stop; r0 += BR, n++) {
       wait_vmcnt<0>();
       block_barrier();
       if (r0 + BR < stop) issue(r0 + BR, n + 1);
-      const int bfirst = r0 / G, blast = min(end - 1, (r0 + BR - 1) / G);
-      if (blast < wfirst || bfirst >= wend) continue;
+      const int w0 = r0 + 32 * rg, wlast_row = min(w0 + 31, stop - 1);
+      const int bfirst = w0 / G, blast = wlast_row / G;
+      if (w0 >= stop || blast < wfirst || bfirst >= wend) continue;
       const bool partial = wj0 + 32 > s.high(a, bfirst) || (wj0 < s.low(a, blast) && wj0 + 32 > a.sinks);
-      const unsigned char* qt = smem + (n & 1) * BUFFER;
+      const unsigned char* qt = smem + (n & 1) * KT::kBuffer;
       const unsigned char* gt = qt + TILE;
-      const float2* stats = reinterpret_cast<const float2*>(gt + TILE);
+      const float2* stats = reinterpret_cast<const float2*>(gt + TILE) + 32 * rg;
+      const int sub = 32 * rg;
+      // The lane's addresses in a tile, computed anew: kept, they would take the registers that the sums need.
+      int at = lane;
+      if constexpr (DP == 128 && sizeof(T) == 2) asm volatile("" : "+v"(at));
+      const int at_col = at & 31, at_hi = at >> 5;
+      floatx16 x = floatx16{};
 #pragma unroll
-      for (int sub = 0; sub < BR; sub += 32) {
-        floatx16 x = floatx16{}, y = floatx16{};
+      for (int kk = 0; kk < STEPS; kk++) x = mma(Tl::nat(qt, sub + at_col, kk, at_hi), kf[kk], x);
+      float p[16];
 #pragma unroll
-        for (int kk = 0; kk < STEPS; kk++) {
-          x = mma(Tl::nat(qt, sub + col, kk, hi), kf[kk], x);
-          y = mma(Tl::nat(gt, sub + col, kk, hi), vf[kk], y);
-        }
-        float p[16], ds[16];
+      for (int v = 0; v < 16; v++)
+        p[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -stats[mfma_row(v, lane)].x));
+      const int2* limits = reinterpret_cast<const int2*>(stats + BR);
+      if (partial) {
 #pragma unroll
         for (int v = 0; v < 16; v++) {
-          const float2 st = stats[sub + mfma_row(v, lane)];
-          p[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -st.x));
-          ds[v] = p[v] * (y[v] - st.y);
+          const int2 lim = limits[mfma_row(v, lane)];
+          if (hidden(key, lim.y, lim.x, a.sinks)) p[v] = 0.0f;
         }
-        if (partial) {
-          const int2* limits = reinterpret_cast<const int2*>(stats + BR);
+      }
+      floatx16 y = floatx16{};
 #pragma unroll
-          for (int v = 0; v < 16; v++) {
-            const int2 lim = limits[sub + mfma_row(v, lane)];
-            if (hidden(key, lim.y, lim.x, a.sinks)) p[v] = ds[v] = 0.0f;
-          }
+      for (int kk = 0; kk < STEPS; kk++) {
+        if constexpr (KT::kShareV) {
+          y = mma(Tl::nat(gt, sub + at_col, kk, at_hi), Tl::nat(vt, 32 * kg + at_col, kk, at_hi), y);
+        } else {
+          y = mma(Tl::nat(gt, sub + at_col, kk, at_hi), vf[kk], y);
         }
-        dk.fit(ds);
+      }
+      // A probability of 0 stays 0 whatever the gradient is.
+      float ds[16];
+#pragma unroll
+      for (int v = 0; v < 16; v++) {
+        const float to = p[v] * (y[v] - stats[mfma_row(v, lane)].y);
+        ds[v] = p[v] == 0.0f ? 0.0f : to;
+      }
+      dk.fit(ds);
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
-          for (int v = 0; v < 16; v++) p[v] *= 0x1p13f;
+          for (int v = 0; v < 8; v++) p[8 * m + v] *= 0x1p13f;
         }
+        const Frag pf = pack8(p + 8 * m, (Frag*)nullptr), df = pack8(ds + 8 * m, (Frag*)nullptr);
 #pragma unroll
-        for (int m = 0; m < 2; m++) {
-          const Frag pf = pack8(p + 8 * m, (Frag*)nullptr), df = pack8(ds + 8 * m, (Frag*)nullptr);
-#pragma unroll
-          for (int c = 0; c < BLOCKS; c++) {
-            dv[c] = mma(Tl::tr(gt, sub + 16 * m, c, lane), pf, dv[c]);
-            dk.acc[c] = mma(Tl::tr(qt, sub + 16 * m, c, lane), df, dk.acc[c]);
-          }
+        for (int c = 0; c < BLOCKS; c++) {
+          dv[c] = mma(Tl::tr(gt, sub + 16 * m, c, at), pf, dv[c]);
+          dk.acc[c] = mma(Tl::tr(qt, sub + 16 * m, c, at), df, dk.acc[c]);
         }
       }
     }
   }
-  if (key >= a.keys) return;
-  const int64_t at = (((int64_t)b * a.keys + key) * a.key_heads + kv) * a.head_dim;
-  T *tk = reinterpret_cast<T*>(a.dk) + at, *tv = reinterpret_cast<T*>(a.dv) + at;
+  // The row groups' sums, in their own magnitude, through LDS: one gradient at a time.
   const float fk = a.scale / dk.scale, fv = sizeof(T) == 2 ? 0x1p-13f : 1.0f;
 #pragma unroll
   for (int c = 0; c < BLOCKS; c++)
 #pragma unroll
-    for (int v = 0; v < 16; v++) {
-      const int ch = 32 * c + mfma_row(v, lane);
+    for (int v = 0; v < 16; v++) dk.acc[c][v] *= fk, dv[c][v] *= fv;
+  static_assert(KT::kRowGroups == 2, "the second group's sums go to the first");
+  float* shared = reinterpret_cast<float*>(smem) + kg * BLOCKS * 1024 + lane;
+  auto meet = [&](floatx16* x) {
+    block_barrier();
+    if (rg == 1) {
+#pragma unroll
+      for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) shared[(16 * c + v) * 64] = x[c][v];
+    }
+    block_barrier();
+    if (rg == 0) {
+#pragma unroll
+      for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) x[c][v] += shared[(16 * c + v) * 64];
+    }
+  };
+  meet(dk.acc);
+  meet(dv);
+  if (rg == 1 || key >= a.keys) return;
+  if (range.chunks > 1) {
+    const int64_t part = ((int64_t)pair * a.tiles + tile) * a.chunks + chunk;
+    float* to = a.partial + (part * 2 * KT::kKeys + 32 * kg + col) * a.head_dim;
+#pragma unroll
+    for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int ch = 32 * c + 8 * g + 4 * hi;
+        if (ch >= a.head_dim) continue;
+#pragma unroll
+        for (int which = 0; which < 2; which++) {
+          const floatx16& x = which ? dv[c] : dk.acc[c];
+          *reinterpret_cast<floatx4*>(to + which * KT::kKeys * a.head_dim + ch) =
+              floatx4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+        }
+      }
+    return;
+  }
+  const int64_t at = (((int64_t)b * a.keys + key) * a.key_heads + kv) * a.head_dim;
+  T *tk = reinterpret_cast<T*>(a.dk) + at, *tv = reinterpret_cast<T*>(a.dv) + at;
+#pragma unroll
+  for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const int ch = 32 * c + 8 * g + 4 * hi;
       if (ch >= a.head_dim) continue;
-      tk[ch] = (T)(live ? dk.acc[c][v] * fk : 0.0f);
-      tv[ch] = (T)(live ? dv[c][v] * fv : 0.0f);
+      const floatx16 &x = dk.acc[c], &y = dv[c];
+      put4(tk + ch, live ? x[4 * g] : 0.0f, live ? x[4 * g + 1] : 0.0f, live ? x[4 * g + 2] : 0.0f,
+           live ? x[4 * g + 3] : 0.0f);
+      put4(tv + ch, live ? y[4 * g] : 0.0f, live ? y[4 * g + 1] : 0.0f, live ? y[4 * g + 2] : 0.0f,
+           live ? y[4 * g + 3] : 0.0f);
     }
 }
 
-template <typename T, int DP> int launch_backward(WindowArgs& a, hipStream_t st) {
+// Adds up the chunks of the tiles that have several, in order: 1,024 values a workgroup.
+template <typename T> __global__ __launch_bounds__(256) void window_dkv_join_kernel(WindowArgs a, int tile_keys, int parts) {
+  const int heads = a.batch * a.key_heads;
+  const int pair = blockIdx.x % heads, rest = blockIdx.x / heads, tile = rest / parts, part = rest % parts;
+  const int b = pair / a.key_heads, kv = pair % a.key_heads, D = a.head_dim;
+  const Sequence s(a, b);
+  const TileRows range(a, s, tile * tile_keys, (tile + 1) * tile_keys);
+  if (range.chunks <= 1) return;
+  const int n = part * 1024 + 4 * (int)threadIdx.x, size = 2 * tile_keys * D;
+  if (n >= size) return;
+  const int which = n >= tile_keys * D, m = n - which * tile_keys * D, key = tile * tile_keys + m / D, ch = m % D;
+  if (key >= a.keys) return;
+  const float* from = a.partial + ((int64_t)pair * a.tiles + tile) * a.chunks * size + n;
+  floatx4 x{};
+#pragma unroll 4
+  for (int c = 0; c < range.chunks; c++) x += *reinterpret_cast<const floatx4*>(from + (int64_t)c * size);
+  if (key >= s.keys) x = floatx4{};
+  T* to = reinterpret_cast<T*>(which ? a.dv : a.dk) + (((int64_t)b * a.keys + key) * a.key_heads + kv) * D + ch;
+  put4(to, x[0], x[1], x[2], x[3]);
+}
+
+// The key tiles, and the rows of a chunk.
+struct KeyPlan {
+  int tile_keys, tiles, chunks, chunk_rows;
+};
+
+KeyPlan key_plan(const afhip_window_desc& d) {
+  KeyPlan p{};
+  const bool wide = d.head_dim > 64 && d.dtype == AFHIP_F32;
+  p.tile_keys = wide ? KeyTile<float, 128>::kKeys : KeyTile<half_t, 128>::kKeys;
+  p.tiles = (int)ceil_div(d.keys, p.tile_keys);
+  const int64_t group = d.query_heads / d.key_heads, all = d.queries * group;
+  // Rows that see a tile, without sinks.
+  const int64_t span = d.left < 0 || d.right < 0
+                           ? all : std::min<int64_t>(all, ((int64_t)d.left + d.right + p.tile_keys) * group);
+  const int64_t most = d.left < 0 || d.sinks > 0 ? all : span, groups = (int64_t)d.batch * d.key_heads * p.tiles;
+  // Two workgroups for each CU, of some blocks of rows.
+  int64_t rows = std::max<int64_t>(ceil_div(span * groups, 512), 512);
+  rows = std::max(rows, ceil_div(most, 64));
+  p.chunk_rows = (int)round_up(rows, 64);
+  p.chunks = (int)ceil_div(most, p.chunk_rows);
+  return p;
+}
+
+size_t chunk_bytes(const afhip_window_desc& d, const KeyPlan& p) {
+  if (p.chunks == 1) return 0;
+  return (size_t)d.batch * d.key_heads * p.tiles * p.chunks * 2 * p.tile_keys * d.head_dim * sizeof(float);
+}
+
+template <typename T, int DP> int launch_backward(WindowArgs& a, const KeyPlan& p, hipStream_t st) {
+  typedef KeyTile<T, DP> KT;
   int s;
   const int64_t heads = (int64_t)a.batch * a.key_heads, rows = (int64_t)a.queries * a.group;
+  AFHIP_REQUIRE(p.tile_keys == KT::kKeys, "key tiles of %d keys, not %d", KT::kKeys, p.tile_keys);
   a.tiles = (int)ceil_div(rows, kHeld);
-  AFHIP_REQUIRE(heads * a.tiles < ((int64_t)1 << 31) && heads * ceil_div(a.keys, kHeld) < ((int64_t)1 << 31),
+  const int parts = (int)ceil_div(2 * KT::kKeys * a.head_dim, 1024);
+  AFHIP_REQUIRE(heads * a.tiles < ((int64_t)1 << 31) && heads * p.tiles * std::max(p.chunks, parts) < ((int64_t)1 << 31),
                 "attention grid too large");
-  constexpr size_t lds_q = 4 * kBlock<T> * DP * sizeof(T), lds_kv = 2 * (2 * kBlock<T> * DP * sizeof(T) + 1024);
+  constexpr size_t lds_q = 4 * kBlock<T> * DP * sizeof(T);
   auto kq = window_dq_kernel<T, DP>;
   if ((s = allow_lds((const void*)kq, lds_q))) return s;
   if ((s = launch("window.dq", kq, dim3((unsigned)(heads * a.tiles)), dim3(64 * kWaves), lds_q, st, a))) return s;
+  a.tiles = p.tiles;
+  a.chunks = p.chunks;
+  a.chunk_rows = p.chunk_rows;
   auto kkv = window_dkv_kernel<T, DP>;
-  if ((s = allow_lds((const void*)kkv, lds_kv))) return s;
-  return launch("window.dkv", kkv, dim3((unsigned)(heads * ceil_div(a.keys, kHeld))), dim3(64 * kWaves), lds_kv, st,
-                a);
+  if ((s = allow_lds((const void*)kkv, KT::kLds))) return s;
+  if ((s = launch("window.dkv", kkv, dim3((unsigned)(heads * p.tiles * p.chunks)), dim3(KT::kThreads), KT::kLds, st, a)))
+    return s;
+  if (p.chunks == 1) return AFHIP_OK;
+  return launch("window.dkv_join", window_dkv_join_kernel<T>, dim3((unsigned)(heads * p.tiles * parts)), dim3(256), 0, st,
+                a, KT::kKeys, parts);
 }
 
-template <typename T> int launch_width(WindowArgs& a, hipStream_t st) {
-  if (a.head_dim <= 32) return launch_backward<T, 32>(a, st);
-  if (a.head_dim <= 64) return launch_backward<T, 64>(a, st);
-  return launch_backward<T, 128>(a, st);
+template <typename T> int launch_width(WindowArgs& a, const KeyPlan& p, hipStream_t st) {
+  if (a.head_dim <= 32) return launch_backward<T, 32>(a, p, st);
+  if (a.head_dim <= 64) return launch_backward<T, 64>(a, p, st);
+  return launch_backward<T, 128>(a, p, st);
 }
 
 size_t row_bytes(const afhip_window_desc& d) {
@@ -363,7 +522,7 @@ extern "C" {
 int afhip_window_backward_workspace_size(const afhip_window_desc* desc, size_t* bytes) {
   if (int s = window_check(desc)) return s;
   AFHIP_REQUIRE(bytes != nullptr, "output is NULL");
-  *bytes = 2 * row_bytes(*desc);
+  *bytes = 2 * row_bytes(*desc) + chunk_bytes(*desc, key_plan(*desc));
   return AFHIP_OK;
 }
 
@@ -405,8 +564,10 @@ int afhip_window_backward(const afhip_window_desc* desc, const void* q, const vo
   a.dv = (char*)dv;
   a.rows = (float2*)workspace;
   a.limits = (int2*)((char*)workspace + row_bytes(d));
+  a.partial = (float*)((char*)workspace + 2 * row_bytes(d));
+  const KeyPlan p = key_plan(d);
   hipStream_t st = (hipStream_t)stream;
-  return d.dtype == AFHIP_F16 ? launch_width<half_t>(a, st) : launch_width<float>(a, st);
+  return d.dtype == AFHIP_F16 ? launch_width<half_t>(a, p, st) : launch_width<float>(a, p, st);
 }
 
 }  // extern "C"
