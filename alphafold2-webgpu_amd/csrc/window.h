@@ -52,13 +52,23 @@ __device__ __forceinline__ floatx16 mma(floatx8 a, floatx8 b, floatx16 c) {
   return c;
 }
 
-// Rows of DP channels (zeros past head_dim) in LDS, 16-byte chunks XORed with their row so that the reads of one
-// column of chunks (nat) and of a few rows (tr) spread over the banks.
+// Rows of DP channels (zeros past head_dim) in LDS, their 16-byte chunks XORed with some of the row's bits, for the 64
+// banks (256 bytes): sixteen rows that are read at one chunk (nat) lie in sixteen different places, and so do the four
+// rows of four chunks of a transposing read (tr): the row's low bits move the groups of four chunks, the next ones the
+// chunks of a group. In f32 a transposed value is read by itself, 32 channels of a row and 32 of the row 4 further on
+// at once: bit 2 of the row moves the groups of eight.
 template <typename T, int DP> struct Tile {
   typedef typename Eight<T>::type Frag;
   static constexpr int kRow = DP * (int)sizeof(T), kChunks = kRow / 16;
 
-  static __device__ __forceinline__ int swizzle(int row) { return kChunks >= 8 ? row & 7 : (row >> 1) & 3; }
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (sizeof(T) == 4) {
+      return kChunks >= 16 ? (row & 3) | ((row & 4) << 1) | ((row & 8) >> 1) : (row >> 1) & 7;
+    } else {
+      const int low = (row >> 2) & 3;
+      return kChunks >= 16 ? ((row & 3) << 2) | low : kChunks == 8 ? ((row & 2) << 1) | low : low;
+    }
+  }
 
   // Channels 16 kk + 8 (lane / 32) .. + 8 of row `row`.
   static __device__ __forceinline__ Frag nat(const unsigned char* t, int row, int kk, int hi) {
@@ -78,53 +88,76 @@ template <typename T, int DP> struct Tile {
   static __device__ __forceinline__ Frag tr(const unsigned char* t, int row0, int cb, int lane) {
     const int hi = lane >> 5;
     if constexpr (sizeof(T) == 2) {
-      const int row = row0 + 4 * hi + ((lane & 15) >> 2);
-      const int ch = 32 * cb + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      const unsigned char* p = t + row * kRow + 16 * ((ch >> 3) ^ swizzle(row)) + 2 * (ch & 7);
-      const window_short4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_window_short4*)p);
-      const window_short4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_window_short4*)(p + 8 * kRow));
+      const int row = 4 * hi + ((lane & 15) >> 2);  // row0 is a multiple of 16, which the swizzle does not see
+      const int chunk = 4 * cb + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      const unsigned char* p = t + row0 * kRow + row * kRow + 8 * (lane & 1);
+      const window_short4 x =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_window_short4*)(p + 16 * (chunk ^ swizzle(row))));
+      const window_short4 y =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_window_short4*)(p + 8 * kRow + 16 * (chunk ^ swizzle(row + 8))));
       return __builtin_bit_cast(half8, window_short8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
     } else {
       const int ch = 32 * cb + (lane & 31);
       Frag f;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const int row = row0 + 4 * hi + (j & 3) + 8 * (j >> 2);
-        f[j] = *reinterpret_cast<const float*>(t + row * kRow + 16 * ((ch >> 2) ^ swizzle(row)) + 4 * (ch & 3));
+        const int row = 4 * hi + (j & 3) + 8 * (j >> 2);
+        f[j] = *reinterpret_cast<const float*>(t + row0 * kRow + row * kRow + 16 * ((ch >> 2) ^ swizzle(row)) +
+                                               4 * (ch & 3));
       }
       return f;
     }
   }
 };
 
-// What a wave loads of a tile of ROWS rows, shared among WAVES waves: which row and byte each lane's chunk of each
-// instruction comes from.
+// What a wave loads of a tile of ROWS rows of a tensor, shared among WAVES waves.
 template <typename T, int DP, int ROWS, int WAVES> struct TileLoad {
   static constexpr int kChunks = Tile<T, DP>::kChunks, kCount = ROWS * kChunks / 64 / WAVES;
   static constexpr int kBytes = ROWS * DP * (int)sizeof(T);
   static_assert(ROWS * kChunks % (64 * WAVES) == 0, "whole instructions for each wave");
 
   static constexpr int kStep = 64 / kChunks;  // rows of an instruction
-  static constexpr int kUnroll = kCount > 8 ? 2 : kCount;
-  int row, chunk, chunks;                     // the lane's row and chunk in a wave's first; a row's chunks
+  // Offsets held for whole tiles, where they are few.
+  static constexpr bool kHeld = kCount <= 4;
+  static constexpr int kUnroll = kHeld ? kCount : 2;
+  int row, chunk, chunks;  // the lane's row and chunk in a wave's first instruction; a row's chunks
+  uint32_t held[kHeld ? kCount : 1];
 
-  __device__ __forceinline__ void init(int wave, int lane, int head_dim) {
+  __device__ __forceinline__ void init(int wave, int lane, int head_dim, int64_t token) {
     row = kStep * wave + lane / kChunks;
     chunk = lane % kChunks;
     chunks = head_dim * (int)sizeof(T) / 16;
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int n = 0; n < kCount; n++) held[n] = at(n, (uint32_t)token);
+    }
+  }
+  __device__ __forceinline__ int row_of(int n) const { return row + kStep * WAVES * n; }
+  // Byte of instruction n's chunk from the tile's first row: at most 127 rows on, of token strides up to 2^24 bytes.
+  __device__ __forceinline__ uint32_t at(int n, uint32_t token) const {
+    const int r = row_of(n), c = chunk ^ Tile<T, DP>::swizzle(r);
+    return c < chunks ? (uint32_t)r * token + 16u * c : kOutOfRange;
   }
 
-  // Rows row0 .. of the tensor at `base`, those that keep(row) holds for; zeros for the others. At most 127 rows
-  // of token strides up to 2^24 bytes after the first: offsets stay below 2^31.
+  // Rows row0 .. of the tensor at `base`: all of them where `whole`, else those that keep(row) holds for and zeros for
+  // the others.
   template <typename Keep>
-  __device__ __forceinline__ void issue(const char* base, int64_t token, int row0, uint32_t lds, int wave,
+  __device__ __forceinline__ void issue(const char* base, int64_t token, int row0, uint32_t lds, int wave, bool whole,
                                         Keep keep) const {
     const int32x4_t rsrc = make_rsrc(base + (int64_t)row0 * token, 0x7ffffff0u);
+    if (whole) {
 #pragma unroll kUnroll
-    for (int n = 0; n < kCount; n++) {
-      const int r = row + kStep * WAVES * n, c = chunk ^ Tile<T, DP>::swizzle(r);
-      const bool ok = (c < chunks) & keep(row0 + r);
-      dma16(rsrc, lds + 1024 * (wave + WAVES * n), ok ? (uint32_t)r * (uint32_t)token + 16u * c : kOutOfRange);
+      for (int n = 0; n < kCount; n++) {
+        if constexpr (kHeld) {
+          dma16(rsrc, lds + 1024 * (wave + WAVES * n), held[n]);
+        } else {
+          dma16(rsrc, lds + 1024 * (wave + WAVES * n), at(n, (uint32_t)token));
+        }
+      }
+    } else {
+#pragma unroll kUnroll
+      for (int n = 0; n < kCount; n++)
+        dma16(rsrc, lds + 1024 * (wave + WAVES * n), keep(row0 + row_of(n)) ? at(n, (uint32_t)token) : kOutOfRange);
     }
   }
 };
@@ -173,10 +206,31 @@ struct Sequence {
   }
 };
 
-// Whether a row that sees keys [low, high) and those below min(sinks, high) does not see `key`: one comparison, so
-// that a block's sixteen tests do not fill the scalar registers with masks.
-__device__ __forceinline__ bool hidden(int key, int low, int high, int sinks) {
-  return min(max(low - key, key - (high - 1)), key - (min(sinks, high) - 1)) > 0;
+// Puts `fill` where a lane's row does not see its sixteen keys from `first` on (its accumulators' rows, mfma_row),
+// seeing keys [low, high) and those below min(sinks, high). ends and starts: whether some row of the wave sees not all
+// of the block for its end or its start, the same for every lane.
+template <typename... X>
+__device__ __forceinline__ void hide(int first, int lane, int low, int high, int sinks, bool ends, bool starts,
+                                     float fill, X&... x) {
+  const int key = first + 4 * (lane >> 5);
+  if (ends) {
+    const int to = high - key;
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+      const bool hidden = 8 * (v >> 2) + (v & 3) >= to;
+      ((x[v] = hidden ? fill : x[v]), ...);
+    }
+  }
+  if (starts) {
+    const int from = low - key, few = sinks - key;
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+      // Of keys not yet hidden: below `low` and not below `sinks`.
+      const int at = 8 * (v >> 2) + (v & 3);
+      const bool hidden = min(from - at, at - few + 1) > 0;
+      ((x[v] = hidden ? fill : x[v]), ...);
+    }
+  }
 }
 
 // The blocks of BK keys that queries first .. last of a sequence see: `sink_blocks` at the start, then `blocks` from
@@ -194,6 +248,23 @@ struct KeyRange {
   }
   __device__ __forceinline__ int block(int t) const { return t < sink_blocks ? t : start + t - sink_blocks; }
   __device__ __forceinline__ bool keeps(int key) const { return (key < high) & ((key >= low) | (key < sinks)); }
+  __device__ __forceinline__ bool whole(int k0, int BK) const {
+    return k0 + BK <= high && (k0 >= low || k0 + BK <= sinks);
+  }
+  // The parts t of [begin, end) that a wave computes, whose rows see keys from any_low to below any_high (and the
+  // sinks): up to `sink_end`, and from `from` to `to`.
+  struct Phases {
+    int sink_end, from, to;
+  };
+  __device__ __forceinline__ Phases phases(int begin, int end, int BK, int any_low, int any_high, bool some) const {
+    Phases p;
+    p.sink_end = some ? min(end, max(begin, sink_blocks)) : begin;
+    // The sinks may reach into the first block of the others.
+    const int first = sinks > start * BK ? start : max(start, any_low / BK);
+    p.from = some ? min(end, max(p.sink_end, first - start + sink_blocks)) : end;
+    p.to = max(p.from, min(end, (any_high + BK - 1) / BK - start + sink_blocks));
+    return p;
+  }
 };
 
 int window_check(const afhip_window_desc* desc);

@@ -60,9 +60,9 @@ template <typename T, int DP> struct Rows {
     low = s.low(a, at);
   }
 
-  // 32 NB keys from k0 on: K and V tiles at kt and vt, `partial` where some row does not see all of them.
+  // 32 NB keys from k0 on: K and V tiles at kt and vt; ends and starts: see hide().
   template <int NB>
-  __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int k0, bool partial,
+  __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int k0, bool ends, bool starts,
                                        int sinks, float scale, int lane) {
     const int col = lane & 31, hi = lane >> 5;
     floatx16 x[NB];
@@ -72,14 +72,9 @@ template <typename T, int DP> struct Rows {
 #pragma unroll
       for (int kk = 0; kk < kSteps; kk++) x[n] = mma(Tile<T, DP>::nat(kt, 32 * n + col, kk, hi), q[kk], x[n]);
     }
-    if (partial) {
+    if (ends | starts) {
 #pragma unroll
-      for (int n = 0; n < NB; n++)
-#pragma unroll
-        for (int v = 0; v < 16; v++) {
-          const int key = k0 + 32 * n + mfma_row(v, lane);
-          if (hidden(key, low, high, sinks)) x[n][v] = -INFINITY;
-        }
+      for (int n = 0; n < NB; n++) hide(k0 + 32 * n, lane, low, high, sinks, ends, starts, -INFINITY, x[n]);
     }
     float top = x[0][0];
 #pragma unroll
@@ -103,6 +98,7 @@ template <typename T, int DP> struct Rows {
       float p[16];
 #pragma unroll
       for (int v = 0; v < 16; v++) p[v] = __builtin_amdgcn_exp2f(fmaf(x[n][v], scale, offset));
+      // Before they are rounded: lse keeps 32 bits.
       l += (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
            (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
 #pragma unroll
@@ -156,30 +152,42 @@ __global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void win
     const int wr0 = r0 + 32 * wave;
     const int wfirst = min(wr0 / a.group, s.queries - 1), wlast = min((wr0 + 31) / a.group, s.queries - 1);
     const int all_low = s.low(a, wlast), all_high = s.high(a, wfirst);
-    const int any_low = s.low(a, wfirst), any_high = s.high(a, wlast);
     const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
     const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
     const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
-    Load load;
-    load.init(wave, lane, a.head_dim);
+    Load kload, vload;
+    kload.init(wave, lane, a.head_dim, a.sk.token);
+    vload.init(wave, lane, a.head_dim, a.sv.token);
     auto issue = [&](int t) {
       const int k0 = range.block(t) * BK;
       const uint32_t buffer = lds + (uint32_t)((t - begin) & 1) * 2 * Load::kBytes;
+      const bool whole = range.whole(k0, BK);
       auto keep = [&](int key) { return range.keeps(key); };
-      load.issue(kb, a.sk.token, k0, buffer, wave, keep);
-      load.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, keep);
+      kload.issue(kb, a.sk.token, k0, buffer, wave, whole, keep);
+      vload.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, whole, keep);
     };
-    if (begin < end) issue(begin);
-    for (int t = begin; t < end; t++) {
-      // Block t is the only one in flight; the barrier publishes it, and every wave is done with block t - 1.
+    // Block t is the only one in flight; the barrier publishes it, and every wave is done with block t - 1.
+    auto arrive = [&](int t) {
       wait_vmcnt<0>();
       block_barrier();
       if (t + 1 < end) issue(t + 1);
-      const int k0 = range.block(t) * BK;
-      if (wr0 >= s.queries * a.group || k0 >= any_high || (k0 + BK <= any_low && k0 >= range.sinks)) continue;
-      const bool partial = k0 + BK > all_high || (k0 < all_low && k0 + BK > range.sinks);
-      const unsigned char* kt = smem + ((t - begin) & 1) * 2 * Load::kBytes;
-      st.template step<BK / 32>(kt, kt + Load::kBytes, k0, partial, range.sinks, a.scale_log2, lane);
+    };
+    if (begin < end) issue(begin);
+    // Blocks that the wave's rows see, between such that only other waves' do. (A branch around the work of one loop
+    // would have the compiler copy all sums at its end.)
+    const auto phases = range.phases(begin, end, BK, s.low(a, wfirst), s.high(a, wlast), wr0 < s.queries * a.group);
+    int t = begin;
+#pragma unroll 1
+    for (int phase = 0; phase < 2; phase++) {
+      const int work = phase ? phases.to : phases.sink_end, idle = phase ? end : phases.from;
+      for (; t < work; t++) {
+        arrive(t);
+        const int k0 = range.block(t) * BK;
+        const unsigned char* kt = smem + ((t - begin) & 1) * 2 * Load::kBytes;
+        st.template step<BK / 32>(kt, kt + Load::kBytes, k0, k0 + BK > all_high, k0 < all_low && k0 + BK > range.sinks,
+                                  range.sinks, a.scale_log2, lane);
+      }
+      for (; t < idle; t++) arrive(t);
     }
   }
   const float l = st.l + __shfl_xor(st.l, 32);
@@ -255,15 +263,17 @@ __global__ __launch_bounds__((kStepThreads<T, DP>)) void window_step_kernel(Wind
     const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
     const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
     const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem) + wave * STAGES * S::kBytes;
-    Load load;
-    load.init(0, lane, a.head_dim);
+    Load kload, vload;
+    kload.init(0, lane, a.head_dim, a.sk.token);
+    vload.init(0, lane, a.head_dim, a.sv.token);
     const int mine = begin + wave < end ? (end - begin - wave + W - 1) / W : 0;
     auto issue = [&](int n) {
       const int k0 = range.block(begin + wave + n * W) * 32;
       const uint32_t buffer = lds + (uint32_t)(n % STAGES) * S::kBytes;
+      const bool whole = range.whole(k0, 32);
       auto keep = [&](int key) { return range.keeps(key); };
-      load.issue(kb, a.sk.token, k0, buffer, 0, keep);
-      load.issue(vb, a.sv.token, k0, buffer + S::kBytes / 2, 0, keep);
+      kload.issue(kb, a.sk.token, k0, buffer, 0, whole, keep);
+      vload.issue(vb, a.sv.token, k0, buffer + S::kBytes / 2, 0, whole, keep);
     };
     for (int n = 0; n < STAGES - 1 && n < mine; n++) issue(n);
     for (int n = 0; n < mine; n++) {
@@ -276,9 +286,9 @@ __global__ __launch_bounds__((kStepThreads<T, DP>)) void window_step_kernel(Wind
         wait_vmcnt<0>();
       }
       const int k0 = range.block(begin + wave + n * W) * 32;
-      const bool partial = k0 + 32 > all_high || (k0 < all_low && k0 + 32 > range.sinks);
       const unsigned char* kt = smem + (wave * STAGES + n % STAGES) * S::kBytes;
-      st.template step<1>(kt, kt + S::kBytes / 2, k0, partial, range.sinks, a.scale_log2, lane);
+      st.template step<1>(kt, kt + S::kBytes / 2, k0, k0 + 32 > all_high, k0 < all_low && k0 + 32 > range.sinks,
+                          range.sinks, a.scale_log2, lane);
     }
   }
   // The waves' reference points, totals and sums: [wave][row][m, l, DP sums].

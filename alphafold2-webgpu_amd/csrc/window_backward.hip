@@ -44,14 +44,12 @@ template <typename T, int BLOCKS> struct Scaled {
         const float both = fmaxf(top, __shfl_xor(top, 32));
         // To [2^7, 2^8).
         const float to = ldexpf(1.0f, min(126, 8 - __builtin_amdgcn_frexp_expf(both)));
-        if (both > 0.0f && to < scale) {
-          const float f = to / scale;
+        const float next = both > 0.0f ? fminf(to, scale) : scale, f = next / scale;
 #pragma unroll
-          for (int c = 0; c < BLOCKS; c++)
+        for (int c = 0; c < BLOCKS; c++)
 #pragma unroll
-            for (int v = 0; v < 16; v++) acc[c][v] *= f;
-          scale = to;
-        }
+          for (int v = 0; v < 16; v++) acc[c][v] *= f;
+        scale = next;
       }
 #pragma unroll
       for (int v = 0; v < 16; v++) ds[v] *= scale;
@@ -114,56 +112,62 @@ __global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void win
     const int wr0 = r0 + 32 * wave;
     const int wfirst = min(wr0 / a.group, s.queries - 1), wlast = min((wr0 + 31) / a.group, s.queries - 1);
     const int all_low = s.low(a, wlast), all_high = s.high(a, wfirst);
-    const int any_low = s.low(a, wfirst), any_high = s.high(a, wlast);
     const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
     const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
     const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
-    Load load;
-    load.init(wave, lane, a.head_dim);
+    Load kload, vload;
+    kload.init(wave, lane, a.head_dim, a.sk.token);
+    vload.init(wave, lane, a.head_dim, a.sv.token);
     auto issue = [&](int t) {
       const int k0 = range.block(t) * BK;
       const uint32_t buffer = lds + (uint32_t)(t & 1) * 2 * Load::kBytes;
+      const bool whole = range.whole(k0, BK);
       auto keep = [&](int key) { return range.keeps(key); };
-      load.issue(kb, a.sk.token, k0, buffer, wave, keep);
-      load.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, keep);
+      kload.issue(kb, a.sk.token, k0, buffer, wave, whole, keep);
+      vload.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, whole, keep);
     };
-    if (range.total > 0) issue(0);
-    for (int t = 0; t < range.total; t++) {
+    auto arrive = [&](int t) {
       wait_vmcnt<0>();
       block_barrier();
       if (t + 1 < range.total) issue(t + 1);
-      const int k0 = range.block(t) * BK;
-      if (wr0 >= s.queries * a.group || k0 >= any_high || (k0 + BK <= any_low && k0 >= range.sinks)) continue;
-      const bool partial = k0 + BK > all_high || (k0 < all_low && k0 + BK > range.sinks);
-      const unsigned char* kt = smem + (t & 1) * 2 * Load::kBytes;
-      const unsigned char* vt = kt + Load::kBytes;
+    };
+    if (range.total > 0) issue(0);
+    // As in window_rows_kernel.
+    const auto phases =
+        range.phases(0, range.total, BK, s.low(a, wfirst), s.high(a, wlast), wr0 < s.queries * a.group);
+    int t = 0;
+#pragma unroll 1
+    for (int phase = 0; phase < 2; phase++) {
+      const int work = phase ? phases.to : phases.sink_end, idle = phase ? range.total : phases.from;
+      for (; t < work; t++) {
+        arrive(t);
+        const int k0 = range.block(t) * BK;
+        const bool ends = k0 + BK > all_high, starts = k0 < all_low && k0 + BK > range.sinks;
+        const unsigned char* kt = smem + (t & 1) * 2 * Load::kBytes;
+        const unsigned char* vt = kt + Load::kBytes;
 #pragma unroll
-      for (int sub = 0; sub < BK; sub += 32) {
-        floatx16 x = floatx16{}, y = floatx16{};
+        for (int sub = 0; sub < BK; sub += 32) {
+          floatx16 x = floatx16{}, y = floatx16{};
 #pragma unroll
-        for (int kk = 0; kk < STEPS; kk++) {
-          x = mma(Tl::nat(kt, sub + col, kk, hi), q[kk], x);
-          y = mma(Tl::nat(vt, sub + col, kk, hi), g[kk], y);
-        }
-        float ds[16];
+          for (int kk = 0; kk < STEPS; kk++) {
+            x = mma(Tl::nat(kt, sub + col, kk, hi), q[kk], x);
+            y = mma(Tl::nat(vt, sub + col, kk, hi), g[kk], y);
+          }
+          float ds[16];
 #pragma unroll
-        for (int v = 0; v < 16; v++)
-          ds[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -lse)) * (y[v] - delta);
-        if (partial) {
+          for (int v = 0; v < 16; v++)
+            ds[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -lse)) * (y[v] - delta);
+          if (ends | starts) hide(k0 + sub, lane, low, high, range.sinks, ends, starts, 0.0f, ds);
+          acc.fit(ds);
 #pragma unroll
-          for (int v = 0; v < 16; v++) {
-            const int key = k0 + sub + mfma_row(v, lane);
-            if (hidden(key, low, high, range.sinks)) ds[v] = 0.0f;
+          for (int n = 0; n < 2; n++) {
+            const Frag f = pack8(ds + 8 * n, (Frag*)nullptr);
+#pragma unroll
+            for (int c = 0; c < BLOCKS; c++) acc.acc[c] = mma(Tl::tr(kt, sub + 16 * n, c, lane), f, acc.acc[c]);
           }
         }
-        acc.fit(ds);
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-          const Frag f = pack8(ds + 8 * n, (Frag*)nullptr);
-#pragma unroll
-          for (int c = 0; c < BLOCKS; c++) acc.acc[c] = mma(Tl::tr(kt, sub + 16 * n, c, lane), f, acc.acc[c]);
-        }
       }
+      for (; t < idle; t++) arrive(t);
     }
   }
   if (row >= rows) return;
@@ -225,7 +229,7 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
   typedef Tile<T, DP> Tl;
   typedef typename Eight<T>::type Frag;
   constexpr int BR = KT::kRows, STEPS = DP / 16, BLOCKS = DP / 32, WAVES = KT::kThreads / 64;
-  constexpr int CHUNKS = Tl::kChunks, STEP = 64 / CHUNKS, COUNT = BR * CHUNKS / 64;
+  constexpr int CHUNKS = Tl::kChunks, STEP = 64 / CHUNKS, COUNT = BR * CHUNKS / 64, UNROLL = sizeof(T) == 2 ? 2 : 1;
   constexpr int TILE = KT::kTileBytes;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
@@ -269,14 +273,19 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
     const float per = 1.0f / (float)G;
     const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
     const int chunks = a.head_dim * (int)sizeof(T) / 16;
+    // Of the block to load next: its first row's query and head.
+    int i0 = begin / G, g0 = begin - i0 * G;
+    const int step_i = BR / G, step_g = BR - step_i * G;
     auto issue = [&](int r0, int n) {
-      // Row r0 + r is query i0 + t / G, head t % G, with t = r + r0 % G: below 2^17, where the rounded quotient of
+      // Row r0 + r is query i0 + t / G, head t % G, with t = r + g0: below 2^17, where the rounded quotient of
       // t + 1/2 has the right whole part.
-      const int i0 = r0 / G, g0 = r0 - i0 * G;
       const int32x4_t qr = make_rsrc(qb + (int64_t)i0 * a.sq.token, 0x7ffffff0u);
       const int32x4_t gr = make_rsrc(gb + (int64_t)i0 * a.sdo.token, 0x7ffffff0u);
       const uint32_t buffer = lds + (uint32_t)(n & 1) * KT::kBuffer;
-      for (int m = wave; m < COUNT; m += WAVES) {
+#pragma unroll UNROLL
+      for (int j = 0; j < (COUNT + WAVES - 1) / WAVES; j++) {
+        const int m = wave + WAVES * j;
+        if (COUNT % WAVES != 0 && m >= COUNT) break;
         const int r = STEP * m + lane / CHUNKS, c = (lane % CHUNKS) ^ Tl::swizzle(r);
         const int t = r + g0, i = (int)(((float)t + 0.5f) * per), g = t - i * G;
         const bool ok = (c < chunks) & (r0 + r < stop);
@@ -294,74 +303,89 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
                                        8u * (uint32_t)max(0, min(32, stop - r0 - part)));
         dma4(sr, buffer + 2 * TILE + 8 * (wave & 1 ? BR : 0) + 8 * part, 4u * lane);
       }
+      i0 += step_i;
+      g0 += step_g;
+      if (g0 >= G) g0 -= G, i0++;
     };
     if constexpr (KT::kShareV) {
       TileLoad<T, DP, KT::kKeys, WAVES> load;
-      load.init(wave, lane, a.head_dim);
-      load.issue(a.v + b * a.sv.batch + kv * a.sv.head, a.sv.token, j0, lds + 2 * KT::kBuffer, wave,
+      load.init(wave, lane, a.head_dim, a.sv.token);
+      load.issue(a.v + b * a.sv.batch + kv * a.sv.head, a.sv.token, j0, lds + 2 * KT::kBuffer, wave, false,
                  [&](int key) { return key < s.keys; });
     }
     issue(begin, 0);
-    int n = 0;
-    for (int r0 = begin; r0 < stop; r0 += BR, n++) {
+    int n = 0, r0 = begin;
+    auto arrive = [&] {
       wait_vmcnt<0>();
       block_barrier();
       if (r0 + BR < stop) issue(r0 + BR, n + 1);
-      const int w0 = r0 + 32 * rg, wlast_row = min(w0 + 31, stop - 1);
-      const int bfirst = w0 / G, blast = wlast_row / G;
-      if (w0 >= stop || blast < wfirst || bfirst >= wend) continue;
-      const bool partial = wj0 + 32 > s.high(a, bfirst) || (wj0 < s.low(a, blast) && wj0 + 32 > a.sinks);
-      const unsigned char* qt = smem + (n & 1) * KT::kBuffer;
-      const unsigned char* gt = qt + TILE;
-      const float2* stats = reinterpret_cast<const float2*>(gt + TILE) + 32 * rg;
-      const int sub = 32 * rg;
-      // The lane's addresses in a tile, computed anew: kept, they would take the registers that the sums need.
-      int at = lane;
-      if constexpr (DP == 128 && sizeof(T) == 2) asm volatile("" : "+v"(at));
-      const int at_col = at & 31, at_hi = at >> 5;
-      floatx16 x = floatx16{};
+    };
+    // Blocks with rows that see the wave's keys, between such that only see other waves'; its own 32 rows of the last
+    // block may be past the end, and are zeros then.
+    const int wbegin = wfirst * G, wstop = min(stop, wend * G);
+    // Rows that see all of them.
+    const int never = rows + 1;
+    const int full_begin =
+        wj0 + 32 > s.keys ? never : a.right < 0 ? 0 : min(rows, max(0, wj0 + 31 - a.right - s.offset) * G);
+    const int full_stop =
+        a.left < 0 || wj0 + 32 <= a.sinks ? never : min(s.queries, max(0, wj0 + a.left - s.offset + 1)) * G;
+#pragma unroll 1
+    for (int phase = 0; phase < 2; phase++) {
+      for (const int idle = phase ? stop : min(stop, wbegin - BR + 1); r0 < idle; r0 += BR, n++) arrive();
+      for (; r0 < wstop; r0 += BR, n++) {
+        arrive();
+        const int w0 = r0 + 32 * rg;
+        const bool partial = w0 < full_begin || min(w0 + 32, stop) > full_stop;
+        const unsigned char* qt = smem + (n & 1) * KT::kBuffer;
+        const unsigned char* gt = qt + TILE;
+        const float2* stats = reinterpret_cast<const float2*>(gt + TILE) + 32 * rg;
+        const int sub = 32 * rg;
+        floatx16 x = floatx16{};
 #pragma unroll
-      for (int kk = 0; kk < STEPS; kk++) x = mma(Tl::nat(qt, sub + at_col, kk, at_hi), kf[kk], x);
-      float p[16];
+        for (int kk = 0; kk < STEPS; kk++) x = mma(Tl::nat(qt, sub + col, kk, hi), kf[kk], x);
+        float p[16];
 #pragma unroll
-      for (int v = 0; v < 16; v++)
-        p[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -stats[mfma_row(v, lane)].x));
-      const int2* limits = reinterpret_cast<const int2*>(stats + BR);
-      if (partial) {
+        for (int v = 0; v < 16; v++)
+          p[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -stats[mfma_row(v, lane)].x));
+        const int2* limits = reinterpret_cast<const int2*>(stats + BR);
+        if (partial) {
+#pragma unroll
+          for (int v = 0; v < 16; v++) {
+            const int2 lim = limits[mfma_row(v, lane)];
+            // As one comparison: a block's sixteen would fill the scalar registers with masks.
+            if (min(max(lim.y - key, key - lim.x + 1), key - min(a.sinks, lim.x) + 1) > 0) p[v] = 0.0f;
+            if (sizeof(T) == 4 && v % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        floatx16 y = floatx16{};
+#pragma unroll
+        for (int kk = 0; kk < STEPS; kk++) {
+          if constexpr (KT::kShareV) {
+            y = mma(Tl::nat(gt, sub + col, kk, hi), Tl::nat(vt, 32 * kg + col, kk, hi), y);
+          } else {
+            y = mma(Tl::nat(gt, sub + col, kk, hi), vf[kk], y);
+          }
+        }
+        // A probability of 0 stays 0 whatever the gradient is.
+        float ds[16];
 #pragma unroll
         for (int v = 0; v < 16; v++) {
-          const int2 lim = limits[mfma_row(v, lane)];
-          if (hidden(key, lim.y, lim.x, a.sinks)) p[v] = 0.0f;
+          const float to = p[v] * (y[v] - stats[mfma_row(v, lane)].y);
+          ds[v] = p[v] == 0.0f ? 0.0f : to;
         }
-      }
-      floatx16 y = floatx16{};
+        dk.fit(ds);
 #pragma unroll
-      for (int kk = 0; kk < STEPS; kk++) {
-        if constexpr (KT::kShareV) {
-          y = mma(Tl::nat(gt, sub + at_col, kk, at_hi), Tl::nat(vt, 32 * kg + at_col, kk, at_hi), y);
-        } else {
-          y = mma(Tl::nat(gt, sub + at_col, kk, at_hi), vf[kk], y);
-        }
-      }
-      // A probability of 0 stays 0 whatever the gradient is.
-      float ds[16];
+        for (int m = 0; m < 2; m++) {
+          if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int v = 0; v < 16; v++) {
-        const float to = p[v] * (y[v] - stats[mfma_row(v, lane)].y);
-        ds[v] = p[v] == 0.0f ? 0.0f : to;
-      }
-      dk.fit(ds);
+            for (int v = 0; v < 8; v++) p[8 * m + v] *= 0x1p13f;
+          }
+          const Frag pf = pack8(p + 8 * m, (Frag*)nullptr), df = pack8(ds + 8 * m, (Frag*)nullptr);
 #pragma unroll
-      for (int m = 0; m < 2; m++) {
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-          for (int v = 0; v < 8; v++) p[8 * m + v] *= 0x1p13f;
-        }
-        const Frag pf = pack8(p + 8 * m, (Frag*)nullptr), df = pack8(ds + 8 * m, (Frag*)nullptr);
-#pragma unroll
-        for (int c = 0; c < BLOCKS; c++) {
-          dv[c] = mma(Tl::tr(gt, sub + 16 * m, c, at), pf, dv[c]);
-          dk.acc[c] = mma(Tl::tr(qt, sub + 16 * m, c, at), df, dk.acc[c]);
+          for (int c = 0; c < BLOCKS; c++) {
+            dv[c] = mma(Tl::tr(gt, sub + 16 * m, c, lane), pf, dv[c]);
+            dk.acc[c] = mma(Tl::tr(qt, sub + 16 * m, c, lane), df, dk.acc[c]);
+          }
         }
       }
     }
@@ -464,7 +488,7 @@ KeyPlan key_plan(const afhip_window_desc& d) {
                            ? all : std::min<int64_t>(all, ((int64_t)d.left + d.right + p.tile_keys) * group);
   const int64_t most = d.left < 0 || d.sinks > 0 ? all : span, groups = (int64_t)d.batch * d.key_heads * p.tiles;
   // Two workgroups for each CU, of some blocks of rows.
-  int64_t rows = std::max<int64_t>(ceil_div(span * groups, 512), 512);
+  int64_t rows = std::max<int64_t>(ceil_div(span * groups, 512), 128);
   rows = std::max(rows, ceil_div(most, 64));
   p.chunk_rows = (int)round_up(rows, 64);
   p.chunks = (int)ceil_div(most, p.chunk_rows);
