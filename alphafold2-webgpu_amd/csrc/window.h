@@ -34,22 +34,56 @@ struct WindowArgs {
 };
 
 typedef float floatx8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short window_short4 __attribute__((ext_vector_type(4)));
 typedef short window_short8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) window_short4 lds_window_short4;
 
-// Eight values along a product's inner axis, a lane's part of 16.
+// Eight values along a product's inner axis, a lane's part of 16. f32 ones are held as three bf16 each, the first 8
+// bits, the next 8 and the last 8, which is all of them: of the nine products of two such values the six that reach
+// 2^-24 of the whole take 192 cycles of the bf16 MFMA, where one of inner length 16 takes 512 of the f32 MFMA.
+struct Parts8 {
+  bf16x8 high, mid, low;
+};
 template <typename T> struct Eight;
 template <> struct Eight<half_t> { typedef half8 type; };
-template <> struct Eight<float> { typedef floatx8 type; };
+template <> struct Eight<float> { typedef Parts8 type; };
+
+__device__ __forceinline__ Parts8 split_parts(floatx8 x) {
+  Parts8 p;
+  u32x4 part[3];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    uint32_t bits[3][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      // Cut, not rounded: the rest is exact and has the value's sign. (An infinity's is NaN: products with it are.)
+      const uint32_t first = __float_as_uint(x[j + i]) & 0xffff0000u;
+      const float rest = x[j + i] - __uint_as_float(first);
+      const uint32_t second = __float_as_uint(rest) & 0xffff0000u;
+      bits[0][i] = first;
+      bits[1][i] = second;
+      bits[2][i] = __float_as_uint(rest - __uint_as_float(second));
+    }
+#pragma unroll
+    for (int n = 0; n < 3; n++) part[n][j / 2] = __builtin_amdgcn_perm(bits[n][1], bits[n][0], 0x07060302u);
+  }
+  p.high = __builtin_bit_cast(bf16x8, part[0]);
+  p.mid = __builtin_bit_cast(bf16x8, part[1]);
+  p.low = __builtin_bit_cast(bf16x8, part[2]);
+  return p;
+}
 
 // acc[32 x 32] += A[32 x 16] B[16 x 32]. Element j of the lane's eight pairs with element j of B's in the same half of
-// the wave; in f32, one MFMA of inner length 2 for each j (a value of each half).
+// the wave.
 __device__ __forceinline__ floatx16 mma(half8 a, half8 b, floatx16 c) { return mfma_f16(a, b, c); }
-__device__ __forceinline__ floatx16 mma(floatx8 a, floatx8 b, floatx16 c) {
-#pragma unroll
-  for (int j = 0; j < 8; j++) c = mfma_f32(a[j], b[j], c);
-  return c;
+__device__ __forceinline__ floatx16 mma(const Parts8& a, const Parts8& b, floatx16 c) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.low, b.high, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.high, b.low, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.mid, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.high, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.high, b.mid, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.high, b.high, c, 0, 0, 0);
 }
 
 // Rows of DP channels (zeros past head_dim) in LDS, their 16-byte chunks XORed with some of the row's bits, for the 64
@@ -79,7 +113,7 @@ template <typename T, int DP> struct Tile {
     } else {
       const floatx4 a = *reinterpret_cast<const floatx4*>(p + 16 * ((4 * kk + 2 * hi) ^ sw));
       const floatx4 b = *reinterpret_cast<const floatx4*>(p + 16 * ((4 * kk + 2 * hi + 1) ^ sw));
-      return floatx8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      return split_parts(floatx8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
     }
   }
 
@@ -98,14 +132,14 @@ template <typename T, int DP> struct Tile {
       return __builtin_bit_cast(half8, window_short8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
     } else {
       const int ch = 32 * cb + (lane & 31);
-      Frag f;
+      floatx8 f;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const int row = 4 * hi + (j & 3) + 8 * (j >> 2);
         f[j] = *reinterpret_cast<const float*>(t + row0 * kRow + row * kRow + 16 * ((ch >> 2) ^ swizzle(row)) +
                                                4 * (ch & 3));
       }
-      return f;
+      return split_parts(f);
     }
   }
 };
@@ -133,10 +167,12 @@ template <typename T, int DP, int ROWS, int WAVES> struct TileLoad {
     }
   }
   __device__ __forceinline__ int row_of(int n) const { return row + kStep * WAVES * n; }
-  // Byte of instruction n's chunk from the tile's first row: at most 127 rows on, of token strides up to 2^24 bytes.
+  // Offsets reach 127 rows, of token strides up to 2^24 bytes: those of a taller tile start anew at each instruction.
+  static constexpr bool kTall = ROWS > 128;
+  static_assert(kStep * WAVES <= 128, "an instruction's rows are in reach");
   __device__ __forceinline__ uint32_t at(int n, uint32_t token) const {
     const int r = row_of(n), c = chunk ^ Tile<T, DP>::swizzle(r);
-    return c < chunks ? (uint32_t)r * token + 16u * c : kOutOfRange;
+    return c < chunks ? (uint32_t)(kTall ? row : r) * token + 16u * c : kOutOfRange;
   }
 
   // Rows row0 .. of the tensor at `base`: all of them where `whole`, else those that keep(row) holds for and zeros for
@@ -144,10 +180,12 @@ template <typename T, int DP, int ROWS, int WAVES> struct TileLoad {
   template <typename Keep>
   __device__ __forceinline__ void issue(const char* base, int64_t token, int row0, uint32_t lds, int wave, bool whole,
                                         Keep keep) const {
-    const int32x4_t rsrc = make_rsrc(base + (int64_t)row0 * token, 0x7ffffff0u);
+    const char* first = base + (int64_t)row0 * token;
+    int32x4_t rsrc = make_rsrc(first, 0x7ffffff0u);
     if (whole) {
 #pragma unroll kUnroll
       for (int n = 0; n < kCount; n++) {
+        if (kTall && n > 0) rsrc = make_rsrc(first + (int64_t)n * kStep * WAVES * token, 0x7ffffff0u);
         if constexpr (kHeld) {
           dma16(rsrc, lds + 1024 * (wave + WAVES * n), held[n]);
         } else {
@@ -155,20 +193,24 @@ template <typename T, int DP, int ROWS, int WAVES> struct TileLoad {
         }
       }
     } else {
-#pragma unroll kUnroll
-      for (int n = 0; n < kCount; n++)
+#pragma unroll 1
+      for (int n = 0; n < kCount; n++) {
+        if (kTall && n > 0) rsrc = make_rsrc(first + (int64_t)n * kStep * WAVES * token, 0x7ffffff0u);
         dma16(rsrc, lds + 1024 * (wave + WAVES * n), keep(row0 + row_of(n)) ? at(n, (uint32_t)token) : kOutOfRange);
+      }
     }
   }
 };
 
 // Eight channels of a row in global memory; zeros where there are none.
-template <typename T> __device__ __forceinline__ typename Eight<T>::type load_eight(const char* row, int channel,
-                                                                                    bool keep) {
-  typename Eight<T>::type f{};
-  if (keep) f = *reinterpret_cast<const typename Eight<T>::type*>(row + channel * (int)sizeof(T));
-  return f;
+__device__ __forceinline__ half8 load_eight(const half_t* p, bool keep) {
+  return keep ? *reinterpret_cast<const half8*>(p) : half8{};
 }
+__device__ __forceinline__ floatx8 load_eight(const float* p, bool keep) {
+  return keep ? *reinterpret_cast<const floatx8*>(p) : floatx8{};
+}
+__device__ __forceinline__ half8 as_fragment(half8 x) { return x; }
+__device__ __forceinline__ Parts8 as_fragment(floatx8 x) { return split_parts(x); }
 
 // Eight accumulators as the second operand of the next product.
 __device__ __forceinline__ half8 pack8(const float* x, half8*) {
@@ -177,8 +219,8 @@ __device__ __forceinline__ half8 pack8(const float* x, half8*) {
   for (int j = 0; j < 8; j++) f[j] = (half_t)x[j];
   return f;
 }
-__device__ __forceinline__ floatx8 pack8(const float* x, floatx8*) {
-  return floatx8{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+__device__ __forceinline__ Parts8 pack8(const float* x, Parts8*) {
+  return split_parts(floatx8{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]});
 }
 
 // Writes four channels.

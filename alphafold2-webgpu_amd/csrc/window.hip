@@ -48,7 +48,7 @@ template <typename T, int DP> struct Rows {
 #pragma unroll
     for (int kk = 0; kk < kSteps; kk++) {
       const int ch = 16 * kk + 8 * hi;
-      q[kk] = load_eight<T>(p, ch, live && ch < a.head_dim);
+      q[kk] = as_fragment(load_eight(reinterpret_cast<const T*>(p) + ch, live && ch < a.head_dim));
     }
 #pragma unroll
     for (int c = 0; c < kBlocks; c++) o[c] = floatx16{};
@@ -120,17 +120,22 @@ __device__ __forceinline__ int64_t lse_index(const WindowArgs& a, int b, int h, 
   return ((int64_t)b * a.query_heads + h) * a.queries + i;
 }
 
-// Four waves of 32 rows over blocks of BK keys that they share through two buffers.
+// Four waves of 32 rows, or with PARTS = 2 eight, of which the second four take the second half of every block: where
+// there are few tiles, twice the waves for the same reads of K and V, and their sums meet in LDS.
 constexpr int kWaves = 4, kTileRows = 32 * kWaves;
-template <typename T> constexpr int kBlockKeys = sizeof(T) == 2 ? 64 : 32;
+template <typename T> constexpr int kBlockKeys = sizeof(T) == 2 ? 64 : 32;  // a wave's, of a block
+template <typename T, int DP, int PARTS> constexpr int kRowsLds = 4 * PARTS * kBlockKeys<T> * DP * (int)sizeof(T);
+// f32 over 128 channels takes more than the 256 registers that eight waves have each.
+template <typename T, int DP> constexpr bool kTwoParts = DP * sizeof(T) <= 256;
 
-template <typename T, int DP, bool SPLIT>
-__global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void window_rows_kernel(WindowArgs a) {
-  constexpr int BK = kBlockKeys<T>;
-  typedef TileLoad<T, DP, BK, kWaves> Load;
+template <typename T, int DP, bool SPLIT, int PARTS>
+__global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) > 256 ? 1 : 2) void window_rows_kernel(
+    WindowArgs a) {
+  constexpr int WK = kBlockKeys<T>, BK = WK * PARTS;
+  typedef TileLoad<T, DP, BK, kWaves * PARTS> Load;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x & 63, hi = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % kWaves, part = wave / kWaves;
   // Neighbours are other key heads (with 8 of them or a multiple, a head's workgroups share an XCD's L2), the last
   // rows first: without a window they see the most keys.
   const int heads = a.batch * a.key_heads;
@@ -139,56 +144,81 @@ __global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void win
   const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
   const Sequence s(a, b);
   const int rows = a.queries * a.group;
-  const int r0 = tile * kTileRows, row = r0 + 32 * wave + (lane & 31);
+  const int r0 = tile * kTileRows, row = r0 + 32 * rg + (lane & 31);
   const int first = r0 / a.group, last = min(s.queries - 1, (r0 + kTileRows - 1) / a.group);
 
+  const KeyRange range(a, s, first, last, BK);
+  const int total = first < s.queries ? range.total : 0;
+  const int begin = SPLIT ? (int)((int64_t)total * split / a.splits) : 0;
+  const int end = SPLIT ? (int)((int64_t)total * (split + 1) / a.splits) : total;
+  // What the wave's rows all see, and what any of them sees.
+  const int wr0 = r0 + 32 * rg;
+  const int wfirst = min(wr0 / a.group, s.queries - 1), wlast = min((wr0 + 31) / a.group, s.queries - 1);
+  const int all_low = s.low(a, wlast), all_high = s.high(a, wfirst);
+  const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
+  const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
+  const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
+  Load kload, vload;
+  kload.init(wave, lane, a.head_dim, a.sk.token);
+  vload.init(wave, lane, a.head_dim, a.sv.token);
+  auto issue = [&](int t) {
+    const int k0 = range.block(t) * BK;
+    const uint32_t buffer = lds + (uint32_t)((t - begin) & 1) * 2 * Load::kBytes;
+    const bool whole = range.whole(k0, BK);
+    auto keep = [&](int key) { return range.keeps(key); };
+    kload.issue(kb, a.sk.token, k0, buffer, wave, whole, keep);
+    vload.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, whole, keep);
+  };
+  // Block t is the only one in flight; the barrier publishes it, and every wave is done with block t - 1.
+  auto arrive = [&](int t) {
+    wait_vmcnt<0>();
+    block_barrier();
+    if (t + 1 < end) issue(t + 1);
+  };
+  // The first keys are on their way before the queries.
+  if (begin < end) issue(begin);
   Rows<T, DP> st;
   st.init(a, s, b, kv, row, hi);
-  if (first < s.queries) {
-    const KeyRange range(a, s, first, last, BK);
-    const int begin = SPLIT ? (int)((int64_t)range.total * split / a.splits) : 0;
-    const int end = SPLIT ? (int)((int64_t)range.total * (split + 1) / a.splits) : range.total;
-    // What the wave's rows all see, and what any of them sees.
-    const int wr0 = r0 + 32 * wave;
-    const int wfirst = min(wr0 / a.group, s.queries - 1), wlast = min((wr0 + 31) / a.group, s.queries - 1);
-    const int all_low = s.low(a, wlast), all_high = s.high(a, wfirst);
-    const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
-    const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
-    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
-    Load kload, vload;
-    kload.init(wave, lane, a.head_dim, a.sk.token);
-    vload.init(wave, lane, a.head_dim, a.sv.token);
-    auto issue = [&](int t) {
-      const int k0 = range.block(t) * BK;
-      const uint32_t buffer = lds + (uint32_t)((t - begin) & 1) * 2 * Load::kBytes;
-      const bool whole = range.whole(k0, BK);
-      auto keep = [&](int key) { return range.keeps(key); };
-      kload.issue(kb, a.sk.token, k0, buffer, wave, whole, keep);
-      vload.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, whole, keep);
-    };
-    // Block t is the only one in flight; the barrier publishes it, and every wave is done with block t - 1.
-    auto arrive = [&](int t) {
-      wait_vmcnt<0>();
-      block_barrier();
-      if (t + 1 < end) issue(t + 1);
-    };
-    if (begin < end) issue(begin);
-    // Blocks that the wave's rows see, between such that only other waves' do. (A branch around the work of one loop
-    // would have the compiler copy all sums at its end.)
-    const auto phases = range.phases(begin, end, BK, s.low(a, wfirst), s.high(a, wlast), wr0 < s.queries * a.group);
-    int t = begin;
+  // Blocks that the wave's rows see, between such that only other waves' do. (A branch around the work of one loop
+  // would have the compiler copy all sums at its end.)
+  const auto phases = range.phases(begin, end, BK, s.low(a, wfirst), s.high(a, wlast), wr0 < s.queries * a.group);
+  int t = begin;
 #pragma unroll 1
-    for (int phase = 0; phase < 2; phase++) {
-      const int work = phase ? phases.to : phases.sink_end, idle = phase ? end : phases.from;
-      for (; t < work; t++) {
-        arrive(t);
-        const int k0 = range.block(t) * BK;
-        const unsigned char* kt = smem + ((t - begin) & 1) * 2 * Load::kBytes;
-        st.template step<BK / 32>(kt, kt + Load::kBytes, k0, k0 + BK > all_high, k0 < all_low && k0 + BK > range.sinks,
-                                  range.sinks, a.scale_log2, lane);
-      }
-      for (; t < idle; t++) arrive(t);
+  for (int phase = 0; phase < 2; phase++) {
+    const int work = phase ? phases.to : phases.sink_end, idle = phase ? end : phases.from;
+    for (; t < work; t++) {
+      arrive(t);
+      const int at = WK * part, k0 = range.block(t) * BK + at;
+      const unsigned char* kt = smem + ((t - begin) & 1) * 2 * Load::kBytes + at * Tile<T, DP>::kRow;
+      st.template step<WK / 32>(kt, kt + Load::kBytes, k0, k0 + WK > all_high, k0 < all_low && k0 + WK > range.sinks,
+                                range.sinks, a.scale_log2, lane);
     }
+    for (; t < idle; t++) arrive(t);
+  }
+  if constexpr (PARTS == 2) {
+    constexpr int VALUES = 2 + DP / 2;
+    static_assert(kWaves * VALUES * 256 <= kRowsLds<T, DP, PARTS>, "the second part's sums fit");
+    float* shared = reinterpret_cast<float*>(smem) + rg * VALUES * 64 + lane;
+    block_barrier();  // the last block is read
+    if (part == 1) {
+      shared[0] = st.m;
+      shared[64] = st.l;
+#pragma unroll
+      for (int c = 0; c < DP / 32; c++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) shared[(2 + 16 * c + v) * 64] = st.o[c][v];
+    }
+    block_barrier();
+    if (part == 1) return;
+    const float other = shared[0], m = fmaxf(st.m, other);
+    const float f = st.m == m ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
+    const float g = other == m ? 1.0f : __builtin_amdgcn_exp2f(other - m);
+    st.m = m;
+    st.l = st.l * f + shared[64] * g;
+#pragma unroll
+    for (int c = 0; c < DP / 32; c++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) st.o[c][v] = st.o[c][v] * f + shared[(2 + 16 * c + v) * 64] * g;
   }
   const float l = st.l + __shfl_xor(st.l, 32);
   if (row >= rows) return;
@@ -227,9 +257,9 @@ __global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void win
   }
 }
 
-// At most 32 rows of a key head (single tokens, or few of them): its waves take blocks of 32 keys in turn, each through
-// buffers of its own, with no barrier until the end, where their sums meet in LDS. What bounds it is the cache's
-// bytes; a split adds workgroups until they fill the card.
+// 32 rows of a key head (single tokens, few of them, or where tiles of 128 rows would leave most CUs without work): its
+// waves take blocks of 32 keys in turn, each through buffers of its own, with no barrier until the end, where their
+// sums meet in LDS. For single tokens the cache's bytes bound it; a split adds workgroups until they fill the card.
 template <typename T, int DP> struct Step {
   static constexpr int kBytes = 2 * 32 * DP * (int)sizeof(T);  // K and V of a block
   static constexpr int kWaves = kBytes >= 32768 ? 2 : 4;
@@ -249,85 +279,86 @@ __global__ __launch_bounds__((kStepThreads<T, DP>)) void window_step_kernel(Wind
   const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = a.batch * a.key_heads;
-  const int pair = blockIdx.x % heads, split = blockIdx.x / heads;
+  const int pair = blockIdx.x % heads, rest = blockIdx.x / heads, tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
   const int b = pair / a.key_heads, kv = pair % a.key_heads;
   const Sequence s(a, b);
-  const int rows = a.queries * a.group;
+  const int all = a.queries * a.group, r0 = 32 * tile, rows = min(32, all - r0);
+  const int first = r0 / a.group, last = min(s.queries - 1, (r0 + rows - 1) / a.group);
   Rows<T, DP> st;
-  st.init(a, s, b, kv, min(col, rows - 1), hi);
-  if (s.queries > 0) {
-    const KeyRange range(a, s, 0, s.queries - 1, 32);
-    const int begin = (int)((int64_t)range.total * split / a.splits);
-    const int end = (int)((int64_t)range.total * (split + 1) / a.splits);
-    const int all_low = s.low(a, s.queries - 1), all_high = s.high(a, 0);
-    const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
-    const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
-    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem) + wave * STAGES * S::kBytes;
-    Load kload, vload;
-    kload.init(0, lane, a.head_dim, a.sk.token);
-    vload.init(0, lane, a.head_dim, a.sv.token);
-    const int mine = begin + wave < end ? (end - begin - wave + W - 1) / W : 0;
-    auto issue = [&](int n) {
-      const int k0 = range.block(begin + wave + n * W) * 32;
-      const uint32_t buffer = lds + (uint32_t)(n % STAGES) * S::kBytes;
-      const bool whole = range.whole(k0, 32);
-      auto keep = [&](int key) { return range.keeps(key); };
-      kload.issue(kb, a.sk.token, k0, buffer, 0, whole, keep);
-      vload.issue(vb, a.sv.token, k0, buffer + S::kBytes / 2, 0, whole, keep);
-    };
-    for (int n = 0; n < STAGES - 1 && n < mine; n++) issue(n);
-    for (int n = 0; n < mine; n++) {
-      // The buffer that block n + STAGES - 1 goes to was read by step n - 1, whose reads have returned.
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (n + STAGES - 1 < mine) {
-        issue(n + STAGES - 1);
-        wait_vmcnt<2 * Load::kCount * (STAGES - 1)>();
-      } else {
-        wait_vmcnt<0>();
-      }
-      const int k0 = range.block(begin + wave + n * W) * 32;
-      const unsigned char* kt = smem + (wave * STAGES + n % STAGES) * S::kBytes;
-      st.template step<1>(kt, kt + S::kBytes / 2, k0, k0 + 32 > all_high, k0 < all_low && k0 + 32 > range.sinks,
-                          range.sinks, a.scale_log2, lane);
+  st.init(a, s, b, kv, r0 + min(col, rows - 1), hi);
+  const KeyRange range(a, s, first, last, 32);
+  const int total = first < s.queries ? range.total : 0;
+  const int begin = (int)((int64_t)total * split / a.splits);
+  const int end = (int)((int64_t)total * (split + 1) / a.splits);
+  const int all_low = s.low(a, last), all_high = s.high(a, first);
+  const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
+  const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
+  const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem) + wave * STAGES * S::kBytes;
+  Load kload, vload;
+  kload.init(0, lane, a.head_dim, a.sk.token);
+  vload.init(0, lane, a.head_dim, a.sv.token);
+  const int mine = begin + wave < end ? (end - begin - wave + W - 1) / W : 0;
+  auto issue = [&](int n) {
+    const int k0 = range.block(begin + wave + n * W) * 32;
+    const uint32_t buffer = lds + (uint32_t)(n % STAGES) * S::kBytes;
+    const bool whole = range.whole(k0, 32);
+    auto keep = [&](int key) { return range.keeps(key); };
+    kload.issue(kb, a.sk.token, k0, buffer, 0, whole, keep);
+    vload.issue(vb, a.sv.token, k0, buffer + S::kBytes / 2, 0, whole, keep);
+  };
+#pragma unroll 1
+  for (int n = 0; n < STAGES - 1 && n < mine; n++) issue(n);
+  for (int n = 0; n < mine; n++) {
+    // The buffer that block n + STAGES - 1 goes to was read by step n - 1, whose reads have returned.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (n + STAGES - 1 < mine) {
+      issue(n + STAGES - 1);
+      wait_vmcnt<2 * Load::kCount * (STAGES - 1)>();
+    } else {
+      wait_vmcnt<0>();
     }
+    const int k0 = range.block(begin + wave + n * W) * 32;
+    const unsigned char* kt = smem + (wave * STAGES + n % STAGES) * S::kBytes;
+    st.template step<1>(kt, kt + S::kBytes / 2, k0, k0 + 32 > all_high, k0 < all_low && k0 + 32 > range.sinks,
+                        range.sinks, a.scale_log2, lane);
   }
   // The waves' reference points, totals and sums: [wave][row][m, l, DP sums].
   float* sums = reinterpret_cast<float*>(smem);
   const float l = st.l + __shfl_xor(st.l, 32);
   block_barrier();  // every wave's loads have landed and been read
   constexpr int PITCH = DP + 2;
-  float* mine = sums + (wave * 32 + col) * PITCH;
+  float* own = sums + (wave * 32 + col) * PITCH;
   if (col < rows) {
-    if (!hi) mine[0] = st.m, mine[1] = l;
+    if (!hi) own[0] = st.m, own[1] = l;
 #pragma unroll
     for (int c = 0; c < DP / 32; c++)
 #pragma unroll
-      for (int v = 0; v < 16; v++) mine[2 + 32 * c + mfma_row(v, lane)] = st.o[c][v];
+      for (int v = 0; v < 16; v++) own[2 + 32 * c + mfma_row(v, lane)] = st.o[c][v];
   }
   block_barrier();
   for (int n = threadIdx.x; n < rows * DP; n += 64 * W) {
     const int r = n / DP, ch = n % DP;
     if (ch >= a.head_dim) continue;
-    float m = -INFINITY, total = 0.0f, o = 0.0f;
+    float m = -INFINITY, sum = 0.0f, o = 0.0f;
 #pragma unroll
     for (int w = 0; w < W; w++) m = fmaxf(m, sums[(w * 32 + r) * PITCH]);
 #pragma unroll
     for (int w = 0; w < W; w++) {
       const float* p = sums + (w * 32 + r) * PITCH;
       const float f = p[0] == m ? 1.0f : __builtin_amdgcn_exp2f(p[0] - m);
-      total += f * p[1];
+      sum += f * p[1];
       o += f * p[2 + ch];
     }
-    const int i = r / a.group, h = kv * a.group + r % a.group;
+    const int i = (r0 + r) / a.group, h = kv * a.group + (r0 + r) % a.group;
     if (a.splits > 1) {
-      float* to = a.partial + (((int64_t)pair * rows + r) * a.splits + split) * (a.head_dim + 2);
+      float* to = a.partial + (((int64_t)pair * all + r0 + r) * a.splits + split) * (a.head_dim + 2);
       to[ch] = o;
-      if (ch == 0) to[a.head_dim] = m, to[a.head_dim + 1] = total;
+      if (ch == 0) to[a.head_dim] = m, to[a.head_dim + 1] = sum;
     } else {
       const bool live = i < s.queries;
       T* to = reinterpret_cast<T*>(a.out + b * a.so.batch + i * a.so.token + h * a.so.head);
-      to[ch] = (T)(live && total != 0.0f ? o / total : 0.0f);
-      if (ch == 0 && a.lse) a.lse[lse_index(a, b, h, i)] = live ? row_lse<T>(m, total) : -INFINITY;
+      to[ch] = (T)(live && sum != 0.0f ? o / sum : 0.0f);
+      if (ch == 0 && a.lse) a.lse[lse_index(a, b, h, i)] = live ? row_lse<T>(m, sum) : -INFINITY;
     }
   }
 }
@@ -377,27 +408,32 @@ template <typename T> __global__ __launch_bounds__(256) void window_join_kernel(
 // Which kernel a call takes, and into how many parts its keys are split.
 struct Plan {
   bool step;
+  int parts;  // of a block of keys, in a workgroup: window_rows_kernel
   int tiles, splits;
 };
 
+const int64_t kFewTiles = getenv("FT") ? atoi(getenv("FT")) : 256;
+const int64_t kWanted = getenv("WT") ? atoi(getenv("WT")) : 512;
+const int64_t kLeast = getenv("LT") ? atoi(getenv("LT")) : 16;
 constexpr int kMaxSplits = 64;  // a lane each in window_join_kernel
 
 Plan plan(const afhip_window_desc& d) {
   const int64_t group = d.query_heads / d.key_heads, rows = d.queries * group, heads = (int64_t)d.batch * d.key_heads;
   Plan p{};
-  p.step = rows <= 32;
-  p.tiles = p.step ? 1 : (int)ceil_div(rows, kTileRows);
+  p.step = rows <= 32 || heads * ceil_div(rows, kTileRows) < kFewTiles;
+  p.tiles = (int)ceil_div(rows, p.step ? 32 : kTileRows);
   // The most keys that a tile's queries see.
   int64_t span = d.keys;
   if (d.left >= 0) {
-    const int64_t queries = p.step ? d.queries : std::min<int64_t>(d.queries, ceil_div(kTileRows, group) + 1);
+    const int64_t queries = std::min<int64_t>(d.queries, ceil_div(p.step ? 32 : kTileRows, group) + 1);
     const int64_t right = d.right < 0 ? d.keys : d.right;
     span = std::min(span, (int64_t)d.left + right + queries + std::min<int64_t>(d.sinks, d.keys));
   }
   const int64_t blocks = ceil_div(span, 32), groups = heads * p.tiles;
-  // Workgroups for every CU, each with a few blocks of keys left.
-  const int64_t wanted = p.step ? 512 : 512, least = p.step ? 16 : 16;
-  int64_t splits = std::min(ceil_div(wanted, groups), blocks / least);
+  // Eight waves for every CU, each with a few blocks of keys left.
+  p.parts = !p.step && groups < 1024 && !(d.dtype == AFHIP_F32 && d.head_dim > 64) ? 2 : 1;
+  const int64_t wanted = p.step ? kWanted : 512 / p.parts;
+  int64_t splits = std::min(ceil_div(wanted, groups), blocks / kLeast);
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
   return p;
 }
@@ -405,6 +441,14 @@ Plan plan(const afhip_window_desc& d) {
 size_t partial_bytes(const afhip_window_desc& d, const Plan& p) {
   if (p.splits == 1) return 0;
   return (size_t)d.batch * d.queries * d.query_heads * p.splits * (d.head_dim + 2) * sizeof(float);
+}
+
+template <typename T, int DP, int PARTS>
+int launch_rows(const WindowArgs& a, const Plan& p, int64_t groups, hipStream_t st) {
+  constexpr size_t lds = kRowsLds<T, DP, PARTS>;
+  auto k = p.splits > 1 ? window_rows_kernel<T, DP, true, PARTS> : window_rows_kernel<T, DP, false, PARTS>;
+  if (int s = allow_lds((const void*)k, lds)) return s;
+  return launch("window.rows", k, dim3((unsigned)groups), dim3(64 * kWaves * PARTS), lds, st, a);
 }
 
 template <typename T, int DP> int launch_forward(const WindowArgs& a, const Plan& p, hipStream_t st) {
@@ -417,10 +461,8 @@ template <typename T, int DP> int launch_forward(const WindowArgs& a, const Plan
     if ((s = allow_lds((const void*)k, S::kLds))) return s;
     s = launch("window.step", k, dim3((unsigned)groups), dim3(64 * S::kWaves), S::kLds, st, a);
   } else {
-    constexpr size_t lds = 4 * kBlockKeys<T> * DP * sizeof(T);
-    auto k = p.splits > 1 ? window_rows_kernel<T, DP, true> : window_rows_kernel<T, DP, false>;
-    if ((s = allow_lds((const void*)k, lds))) return s;
-    s = launch("window.rows", k, dim3((unsigned)groups), dim3(64 * kWaves), lds, st, a);
+    s = p.parts == 2 ? launch_rows<T, DP, kTwoParts<T, DP> ? 2 : 1>(a, p, groups, st)
+                     : launch_rows<T, DP, 1>(a, p, groups, st);
   }
   if (s || p.splits == 1) return s;
   const int64_t rows = (int64_t)a.batch * a.queries * a.query_heads;

@@ -14,6 +14,7 @@
 // the accumulators are rescaled with it.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "window.h"
 
@@ -21,7 +22,6 @@ namespace afhip {
 
 namespace {
 
-constexpr int kWaves = 4, kHeld = 32 * kWaves;
 template <typename T> constexpr int kBlock = sizeof(T) == 2 ? 64 : 32;  // keys or rows of a streamed block
 
 // A held row's power of two on ds (f16), and the accumulators it is on.
@@ -57,26 +57,64 @@ template <typename T, int BLOCKS> struct Scaled {
   }
 };
 
-// dq, and each row's lse and D for the other kernel. Rows as in window_rows_kernel.
-template <typename T, int DP>
-__global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void window_dq_kernel(WindowArgs a) {
-  constexpr int BK = kBlock<T>, STEPS = DP / 16, BLOCKS = DP / 32;
-  typedef TileLoad<T, DP, BK, kWaves> Load;
+// dq, and each row's lse and D for the other kernel. ROWS waves of 32 rows each, and PARTS times as many where there
+// are few rows: each part takes its WK keys of every block, and the parts' sums meet in LDS.
+template <typename T, int DP, int ROWS, int PARTS, int WK> struct RowTile {
+  static constexpr int kRows = 32 * ROWS, kThreads = 64 * ROWS * PARTS;
+  static constexpr int kLds = 4 * PARTS * WK * DP * (int)sizeof(T);
+  // Workgroups a CU, for its LDS; the widest f32 takes more than 256 registers.
+  static constexpr int kGroups = kLds > 81920 || DP * sizeof(T) > 256 ? 1 : 2;
+  static_assert(PARTS == 1 || (PARTS - 1) * ROWS * DP * 128 <= kLds, "the other parts' sums fit");
+};
+
+template <typename T, int DP, int ROWS, int PARTS, int WK>
+__global__ __launch_bounds__((RowTile<T, DP, ROWS, PARTS, WK>::kThreads), (RowTile<T, DP, ROWS, PARTS, WK>::kGroups)) void
+window_dq_kernel(WindowArgs a) {
+  constexpr int BK = WK * PARTS, STEPS = DP / 16, BLOCKS = DP / 32;
+  constexpr int HELD = RowTile<T, DP, ROWS, PARTS, WK>::kRows;
+  typedef TileLoad<T, DP, BK, ROWS * PARTS> Load;
   typedef typename Eight<T>::type Frag;
   typedef Tile<T, DP> Tl;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % ROWS, part = wave / ROWS;
   const int heads = a.batch * a.key_heads;
   const int pair = blockIdx.x % heads, tile = a.tiles - 1 - blockIdx.x / heads;
   const int b = pair / a.key_heads, kv = pair % a.key_heads;
   const Sequence s(a, b);
   const int rows = a.queries * a.group;
-  const int r0 = tile * kHeld, row = r0 + 32 * wave + col;
-  const int first = r0 / a.group, last = min(s.queries - 1, (r0 + kHeld - 1) / a.group);
+  const int r0 = tile * HELD, row = r0 + 32 * rg + col;
+  const int first = r0 / a.group, last = min(s.queries - 1, (r0 + HELD - 1) / a.group);
   const int i = row / a.group, h = kv * a.group + row % a.group;
   const bool live = i < s.queries;
   const int at = min(i, s.queries - 1), high = s.high(a, at), low = s.low(a, at);
+
+  // The first keys are on their way before all else.
+  const KeyRange range(a, s, first, last, BK);
+  const int total = first < s.queries ? range.total : 0;
+  const int wr0 = r0 + 32 * rg;
+  const int wfirst = min(wr0 / a.group, s.queries - 1), wlast = min((wr0 + 31) / a.group, s.queries - 1);
+  const int all_low = s.low(a, wlast), all_high = s.high(a, wfirst);
+  const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
+  const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
+  const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
+  Load kload, vload;
+  kload.init(wave, lane, a.head_dim, a.sk.token);
+  vload.init(wave, lane, a.head_dim, a.sv.token);
+  auto issue = [&](int t) {
+    const int k0 = range.block(t) * BK;
+    const uint32_t buffer = lds + (uint32_t)(t & 1) * 2 * Load::kBytes;
+    const bool whole = range.whole(k0, BK);
+    auto keep = [&](int key) { return range.keeps(key); };
+    kload.issue(kb, a.sk.token, k0, buffer, wave, whole, keep);
+    vload.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, whole, keep);
+  };
+  auto arrive = [&](int t) {
+    wait_vmcnt<0>();
+    block_barrier();
+    if (t + 1 < total) issue(t + 1);
+  };
+  if (total > 0) issue(0);
 
   Frag q[STEPS], g[STEPS];
   float delta = 0.0f, lse = INFINITY;
@@ -89,96 +127,96 @@ __global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void win
     for (int kk = 0; kk < STEPS; kk++) {
       const int ch = 16 * kk + 8 * hi;
       const bool keep = live && ch < a.head_dim;
-      q[kk] = load_eight<T>(qp, ch, keep);
-      g[kk] = load_eight<T>(gp, ch, keep);
-      const Frag o = load_eight<T>(op, ch, keep);
+      q[kk] = as_fragment(load_eight(reinterpret_cast<const T*>(qp) + ch, keep));
+      const auto y = load_eight(reinterpret_cast<const T*>(gp) + ch, keep);
+      const auto o = load_eight(reinterpret_cast<const T*>(op) + ch, keep);
+      g[kk] = as_fragment(y);
 #pragma unroll
-      for (int j = 0; j < 8; j++) delta += (float)o[j] * (float)g[kk][j];
+      for (int j = 0; j < 8; j++) delta += (float)o[j] * (float)y[j];
     }
     delta += __shfl_xor(delta, 32);
     if (live) {
       lse = a.lse[((int64_t)b * a.query_heads + h) * a.queries + i] * kWindowLog2e;
       if (lse == -INFINITY) lse = INFINITY;  // nothing seen: probabilities of 0
     }
-    if (row < rows && !hi) {
+    if (row < rows && !hi && part == 0) {
       a.rows[(int64_t)pair * rows + row] = float2{lse, delta};
       a.limits[(int64_t)pair * rows + row] = live ? int2{high, low} : int2{0, 0};
     }
   }
   Scaled<T, BLOCKS> acc;
   acc.init();
-  if (first < s.queries) {
-    const KeyRange range(a, s, first, last, BK);
-    const int wr0 = r0 + 32 * wave;
-    const int wfirst = min(wr0 / a.group, s.queries - 1), wlast = min((wr0 + 31) / a.group, s.queries - 1);
-    const int all_low = s.low(a, wlast), all_high = s.high(a, wfirst);
-    const char* kb = a.k + b * a.sk.batch + kv * a.sk.head;
-    const char* vb = a.v + b * a.sv.batch + kv * a.sv.head;
-    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
-    Load kload, vload;
-    kload.init(wave, lane, a.head_dim, a.sk.token);
-    vload.init(wave, lane, a.head_dim, a.sv.token);
-    auto issue = [&](int t) {
-      const int k0 = range.block(t) * BK;
-      const uint32_t buffer = lds + (uint32_t)(t & 1) * 2 * Load::kBytes;
-      const bool whole = range.whole(k0, BK);
-      auto keep = [&](int key) { return range.keeps(key); };
-      kload.issue(kb, a.sk.token, k0, buffer, wave, whole, keep);
-      vload.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, whole, keep);
-    };
-    auto arrive = [&](int t) {
-      wait_vmcnt<0>();
-      block_barrier();
-      if (t + 1 < range.total) issue(t + 1);
-    };
-    if (range.total > 0) issue(0);
-    // As in window_rows_kernel.
-    const auto phases =
-        range.phases(0, range.total, BK, s.low(a, wfirst), s.high(a, wlast), wr0 < s.queries * a.group);
-    int t = 0;
+  // As in window_rows_kernel.
+  const auto phases =
+      range.phases(0, total, BK, s.low(a, wfirst), s.high(a, wlast), wr0 < s.queries * a.group);
+  int t = 0;
 #pragma unroll 1
-    for (int phase = 0; phase < 2; phase++) {
-      const int work = phase ? phases.to : phases.sink_end, idle = phase ? range.total : phases.from;
-      for (; t < work; t++) {
-        arrive(t);
-        const int k0 = range.block(t) * BK;
-        const bool ends = k0 + BK > all_high, starts = k0 < all_low && k0 + BK > range.sinks;
-        const unsigned char* kt = smem + (t & 1) * 2 * Load::kBytes;
-        const unsigned char* vt = kt + Load::kBytes;
+  for (int phase = 0; phase < 2; phase++) {
+    const int work = phase ? phases.to : phases.sink_end, idle = phase ? total : phases.from;
+    for (; t < work; t++) {
+      arrive(t);
+      const int at = WK * part, k0 = range.block(t) * BK + at;
+      const bool ends = k0 + WK > all_high, starts = k0 < all_low && k0 + WK > range.sinks;
+      const unsigned char* kt = smem + (t & 1) * 2 * Load::kBytes + at * Tl::kRow;
+      const unsigned char* vt = kt + Load::kBytes;
 #pragma unroll
-        for (int sub = 0; sub < BK; sub += 32) {
-          floatx16 x = floatx16{}, y = floatx16{};
+      for (int sub = 0; sub < WK; sub += 32) {
+        floatx16 x = floatx16{}, y = floatx16{};
 #pragma unroll
-          for (int kk = 0; kk < STEPS; kk++) {
-            x = mma(Tl::nat(kt, sub + col, kk, hi), q[kk], x);
-            y = mma(Tl::nat(vt, sub + col, kk, hi), g[kk], y);
-          }
-          float ds[16];
+        for (int kk = 0; kk < STEPS; kk++) {
+          x = mma(Tl::nat(kt, sub + col, kk, hi), q[kk], x);
+          y = mma(Tl::nat(vt, sub + col, kk, hi), g[kk], y);
+        }
+        float ds[16];
 #pragma unroll
-          for (int v = 0; v < 16; v++)
-            ds[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -lse)) * (y[v] - delta);
-          if (ends | starts) hide(k0 + sub, lane, low, high, range.sinks, ends, starts, 0.0f, ds);
-          acc.fit(ds);
+        for (int v = 0; v < 16; v++)
+          ds[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -lse)) * (y[v] - delta);
+        if (ends | starts) hide(k0 + sub, lane, low, high, range.sinks, ends, starts, 0.0f, ds);
+        acc.fit(ds);
 #pragma unroll
-          for (int n = 0; n < 2; n++) {
-            const Frag f = pack8(ds + 8 * n, (Frag*)nullptr);
+        for (int n = 0; n < 2; n++) {
+          const Frag f = pack8(ds + 8 * n, (Frag*)nullptr);
 #pragma unroll
-            for (int c = 0; c < BLOCKS; c++) acc.acc[c] = mma(Tl::tr(kt, sub + 16 * n, c, lane), f, acc.acc[c]);
-          }
+          for (int c = 0; c < BLOCKS; c++) acc.acc[c] = mma(Tl::tr(kt, sub + 16 * n, c, lane), f, acc.acc[c]);
         }
       }
-      for (; t < idle; t++) arrive(t);
     }
+    for (; t < idle; t++) arrive(t);
   }
-  if (row >= rows) return;
-  T* to = reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.queries + i) * a.query_heads + h) * a.head_dim;
   const float f = a.scale / acc.scale;
 #pragma unroll
   for (int c = 0; c < BLOCKS; c++)
 #pragma unroll
-    for (int v = 0; v < 16; v++) {
-      const int ch = 32 * c + mfma_row(v, lane);
-      if (ch < a.head_dim) to[ch] = (T)(live ? acc.acc[c][v] * f : 0.0f);
+    for (int v = 0; v < 16; v++) acc.acc[c][v] *= f;
+  if constexpr (PARTS > 1) {
+    float* shared = reinterpret_cast<float*>(smem) + rg * BLOCKS * 1024 + lane;
+    block_barrier();  // the last block is read
+    if (part > 0) {
+#pragma unroll
+      for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) shared[((part - 1) * ROWS * BLOCKS * 16 + 16 * c + v) * 64] = acc.acc[c][v];
+    }
+    block_barrier();
+    if (part > 0) return;
+#pragma unroll 1
+    for (int p = 0; p < PARTS - 1; p++)
+#pragma unroll
+      for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) acc.acc[c][v] += shared[(p * ROWS * BLOCKS * 16 + 16 * c + v) * 64];
+  }
+  if (row >= rows) return;
+  T* to = reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.queries + i) * a.query_heads + h) * a.head_dim;
+#pragma unroll
+  for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const int ch = 32 * c + 8 * g + 4 * hi;
+      if (ch >= a.head_dim) continue;
+      const floatx16& x = acc.acc[c];
+      put4(to + ch, live ? x[4 * g] : 0.0f, live ? x[4 * g + 1] : 0.0f, live ? x[4 * g + 2] : 0.0f,
+           live ? x[4 * g + 3] : 0.0f);
     }
 }
 
@@ -190,7 +228,9 @@ __global__ __launch_bounds__(64 * kWaves, DP * sizeof(T) > 256 ? 1 : 2) void win
 // Tiles differ in how many rows see them (those of the sinks: all), and few sequences have few tiles: the rows are cut
 // into chunks, and a tile of several leaves partial sums, joined by window_dkv_join_kernel.
 template <typename T, int DP> struct KeyTile {
-  static constexpr int kKeyGroups = DP * sizeof(T) > 256 ? 2 : 4, kRowGroups = 2, kThreads = 64 * kKeyGroups * kRowGroups;
+  // Values of three bf16 take more than the 256 registers that eight waves have each from 64 channels on.
+  static constexpr int kKeyGroups = sizeof(T) == 4 && DP > 32 ? 2 : 4, kRowGroups = 2;
+  static constexpr int kThreads = 64 * kKeyGroups * kRowGroups;
   static constexpr int kKeys = 32 * kKeyGroups, kRows = 32 * kRowGroups;
   static constexpr int kStats = 16 * kRows;  // the rows' statistics and limits
   static constexpr int kTileBytes = kRows * DP * (int)sizeof(T), kBuffer = 2 * kTileBytes + kStats;
@@ -246,18 +286,6 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
   if (chunk > 0 && chunk >= range.chunks) return;
   const int begin = range.begin + chunk * a.chunk_rows, stop = min(range.stop, begin + a.chunk_rows);
 
-  Frag kf[STEPS], vf[KT::kShareV ? 1 : STEPS];
-  {
-    const int64_t src = live ? key : 0;
-    const char* kp = a.k + b * a.sk.batch + src * a.sk.token + kv * a.sk.head;
-    const char* vp = a.v + b * a.sv.batch + src * a.sv.token + kv * a.sv.head;
-#pragma unroll
-    for (int kk = 0; kk < STEPS; kk++) {
-      const int ch = 16 * kk + 8 * hi;
-      kf[kk] = load_eight<T>(kp, ch, live && ch < a.head_dim);
-      if constexpr (!KT::kShareV) vf[kk] = load_eight<T>(vp, ch, live && ch < a.head_dim);
-    }
-  }
   const unsigned char* vt = smem + 2 * KT::kBuffer;
   Scaled<T, BLOCKS> dk;
   floatx16 dv[BLOCKS];
@@ -313,6 +341,37 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
       load.issue(a.v + b * a.sv.batch + kv * a.sv.head, a.sv.token, j0, lds + 2 * KT::kBuffer, wave, false,
                  [&](int key) { return key < s.keys; });
     }
+    // Over 128 channels of f32 K and V are held as they are, and made three bf16 at each use, which costs a tenth of the
+    // MFMAs' time: as parts they would not fit.
+    constexpr bool RAW = sizeof(T) == 4 && DP == 128;
+    typedef typename std::conditional<RAW, floatx8, Frag>::type Held;
+    Held kf[STEPS], vf[KT::kShareV ? 1 : STEPS];
+    auto held = [](Held& x) {
+      if constexpr (RAW) {
+        asm volatile("" : "+v"(x));  // not ahead of the loop
+        return split_parts(x);
+      } else {
+        return x;
+      }
+    };
+    {
+      const int64_t src = live ? key : 0;
+      const char* kp = a.k + b * a.sk.batch + src * a.sk.token + kv * a.sk.head;
+      const char* vp = a.v + b * a.sv.batch + src * a.sv.token + kv * a.sv.head;
+#pragma unroll
+      for (int kk = 0; kk < STEPS; kk++) {
+        const int ch = 16 * kk + 8 * hi;
+        const bool keep = live && ch < a.head_dim;
+        const auto x = load_eight(reinterpret_cast<const T*>(kp) + ch, keep);
+        if constexpr (RAW) {
+          kf[kk] = x;
+          vf[kk] = load_eight(reinterpret_cast<const T*>(vp) + ch, keep);
+        } else {
+          kf[kk] = as_fragment(x);
+          if constexpr (!KT::kShareV) vf[kk] = as_fragment(load_eight(reinterpret_cast<const T*>(vp) + ch, keep));
+        }
+      }
+    }
     issue(begin, 0);
     int n = 0, r0 = begin;
     auto arrive = [&] {
@@ -342,7 +401,7 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
         const int sub = 32 * rg;
         floatx16 x = floatx16{};
 #pragma unroll
-        for (int kk = 0; kk < STEPS; kk++) x = mma(Tl::nat(qt, sub + col, kk, hi), kf[kk], x);
+        for (int kk = 0; kk < STEPS; kk++) x = mma(Tl::nat(qt, sub + col, kk, hi), held(kf[kk]), x);
         float p[16];
 #pragma unroll
         for (int v = 0; v < 16; v++)
@@ -363,7 +422,7 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
           if constexpr (KT::kShareV) {
             y = mma(Tl::nat(gt, sub + col, kk, hi), Tl::nat(vt, 32 * kg + col, kk, hi), y);
           } else {
-            y = mma(Tl::nat(gt, sub + col, kk, hi), vf[kk], y);
+            y = mma(Tl::nat(gt, sub + col, kk, hi), held(vf[kk]), y);
           }
         }
         // A probability of 0 stays 0 whatever the gradient is.
@@ -479,7 +538,7 @@ struct KeyPlan {
 
 KeyPlan key_plan(const afhip_window_desc& d) {
   KeyPlan p{};
-  const bool wide = d.head_dim > 64 && d.dtype == AFHIP_F32;
+  const bool wide = d.head_dim > 32 && d.dtype == AFHIP_F32;
   p.tile_keys = wide ? KeyTile<float, 128>::kKeys : KeyTile<half_t, 128>::kKeys;
   p.tiles = (int)ceil_div(d.keys, p.tile_keys);
   const int64_t group = d.query_heads / d.key_heads, all = d.queries * group;
@@ -500,19 +559,35 @@ size_t chunk_bytes(const afhip_window_desc& d, const KeyPlan& p) {
   return (size_t)d.batch * d.key_heads * p.tiles * p.chunks * 2 * p.tile_keys * d.head_dim * sizeof(float);
 }
 
+template <typename T, int DP, int ROWS, int PARTS, int WK>
+int launch_dq(WindowArgs& a, int64_t heads, int64_t rows, hipStream_t st) {
+  typedef RowTile<T, DP, ROWS, PARTS, WK> RT;
+  a.tiles = (int)ceil_div(rows, RT::kRows);
+  AFHIP_REQUIRE(heads * a.tiles < ((int64_t)1 << 31), "attention grid too large");
+  auto k = window_dq_kernel<T, DP, ROWS, PARTS, WK>;
+  if (int s = allow_lds((const void*)k, RT::kLds)) return s;
+  return launch("window.dq", k, dim3((unsigned)(heads * a.tiles)), dim3(RT::kThreads), RT::kLds, st, a);
+}
+
+// Tiles of 128 rows with four waves, or with eight where that would leave CUs with fewer, or of 32 rows where those
+// would leave most CUs with nothing.
+template <typename T, int DP> int launch_dq_any(WindowArgs& a, int64_t heads, int64_t rows, hipStream_t st) {
+  constexpr int WK = kBlock<T>, EIGHT = DP * sizeof(T) > 256 ? 1 : 2;
+  constexpr int FEW = DP * sizeof(T) > 256 ? 2 : DP * sizeof(T) > 64 ? 4 : 8;
+  const int64_t groups = heads * ceil_div(rows, 128);
+  if (groups < 128) return launch_dq<T, DP, 1, FEW, 32>(a, heads, rows, st);
+  if (groups < 512) return launch_dq<T, DP, 4, EIGHT, WK>(a, heads, rows, st);
+  return launch_dq<T, DP, 4, 1, WK>(a, heads, rows, st);
+}
+
 template <typename T, int DP> int launch_backward(WindowArgs& a, const KeyPlan& p, hipStream_t st) {
   typedef KeyTile<T, DP> KT;
   int s;
   const int64_t heads = (int64_t)a.batch * a.key_heads, rows = (int64_t)a.queries * a.group;
   AFHIP_REQUIRE(p.tile_keys == KT::kKeys, "key tiles of %d keys, not %d", KT::kKeys, p.tile_keys);
-  a.tiles = (int)ceil_div(rows, kHeld);
   const int parts = (int)ceil_div(2 * KT::kKeys * a.head_dim, 1024);
-  AFHIP_REQUIRE(heads * a.tiles < ((int64_t)1 << 31) && heads * p.tiles * std::max(p.chunks, parts) < ((int64_t)1 << 31),
-                "attention grid too large");
-  constexpr size_t lds_q = 4 * kBlock<T> * DP * sizeof(T);
-  auto kq = window_dq_kernel<T, DP>;
-  if ((s = allow_lds((const void*)kq, lds_q))) return s;
-  if ((s = launch("window.dq", kq, dim3((unsigned)(heads * a.tiles)), dim3(64 * kWaves), lds_q, st, a))) return s;
+  AFHIP_REQUIRE(heads * p.tiles * std::max(p.chunks, parts) < ((int64_t)1 << 31), "attention grid too large");
+  if ((s = launch_dq_any<T, DP>(a, heads, rows, st))) return s;
   a.tiles = p.tiles;
   a.chunks = p.chunks;
   a.chunk_rows = p.chunk_rows;
