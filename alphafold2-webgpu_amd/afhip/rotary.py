@@ -150,7 +150,7 @@ class HeadRotary:
         into a cache. q_out may be q, and k_out k."""
         import torch
 
-        if torch.cuda.current_device() != self._device:
+        if _current_device() != self._device:
             with torch.cuda.device(self._device):
                 return self(q, k, v, past=past, lengths=lengths, positions=positions, q_out=q_out, k_out=k_out,
                             k_cache=k_cache, v_cache=v_cache)
@@ -206,7 +206,7 @@ class HeadRotary:
         "dkey_scale", with "layer" "dquery_offset" and "dkey_offset" too (f32 [head_dim])."""
         import torch
 
-        if torch.cuda.current_device() != self._device:
+        if _current_device() != self._device:
             with torch.cuda.device(self._device):
                 return self.backward(q, k, dq_out, dk_out, past=past, lengths=lengths, positions=positions)
         self._ready()

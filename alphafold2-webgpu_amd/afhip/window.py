@@ -76,7 +76,7 @@ class WindowAttention:
         read."""
         import torch
 
-        if torch.cuda.current_device() != self._device:
+        if _current_device() != self._device:
             with torch.cuda.device(self._device):
                 return self(q, k, v, query_lengths=query_lengths, key_lengths=key_lengths, out=out,
                             return_lse=return_lse)
@@ -106,7 +106,7 @@ class WindowAttention:
         the query heads that read them. Zeros past the lengths. The same bits at every call."""
         import torch
 
-        if torch.cuda.current_device() != self._device:
+        if _current_device() != self._device:
             with torch.cuda.device(self._device):
                 return self.backward(q, k, v, out, lse, dout, query_lengths=query_lengths, key_lengths=key_lengths)
         key = ("backward", form(q), form(k), form(v), form(out), form(lse), form(dout), form(query_lengths),

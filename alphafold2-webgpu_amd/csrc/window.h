@@ -30,7 +30,9 @@ struct WindowArgs {
   // [batch][key head][row]: the row's lse in base 2 and the sum of out * dout; the keys it sees, below and from.
   float2* rows;
   int2* limits;
-  int chunks, chunk_rows;  // dk and dv: the most chunks of rows that a tile of keys has, and the rows of one
+  // dk and dv: the most chunks of rows that a tile of keys has, the rows of one; tiles that all rows may see, and the
+  // chunks of the others.
+  int chunks, chunk_rows, long_tiles, short_chunks;
 };
 
 typedef float floatx8 __attribute__((ext_vector_type(8)));
@@ -229,6 +231,13 @@ __device__ __forceinline__ void put4(half_t* p, float a, float b, float c, float
 }
 __device__ __forceinline__ void put4(float* p, float a, float b, float c, float d) {
   *reinterpret_cast<floatx4*>(p) = floatx4{a, b, c, d};
+}
+
+// Of two waves on a SIMD one goes first wherever both could issue, so that its MFMAs run beside the other's vector
+// instructions and not in step with them: the waves' slots tell them apart.
+__device__ __forceinline__ void prefer_one_of_two() {
+  constexpr int kWaveSlot = 4 | (0 << 6) | (3 << 11);  // HW_ID, bits 0 to 3
+  if (__builtin_amdgcn_s_getreg(kWaveSlot) & 1) __builtin_amdgcn_s_setprio(1);
 }
 
 // One sequence: its numbers of queries and keys, and where its queries start.

@@ -134,6 +134,7 @@ __global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) >
   constexpr int WK = kBlockKeys<T>, BK = WK * PARTS;
   typedef TileLoad<T, DP, BK, kWaves * PARTS> Load;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  prefer_one_of_two();
   const int lane = threadIdx.x & 63, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % kWaves, part = wave / kWaves;
   // Neighbours are other key heads (with 8 of them or a multiple, a head's workgroups share an XCD's L2), the last
@@ -412,16 +413,21 @@ struct Plan {
   int tiles, splits;
 };
 
-const int64_t kFewTiles = getenv("FT") ? atoi(getenv("FT")) : 256;
-const int64_t kWanted = getenv("WT") ? atoi(getenv("WT")) : 512;
-const int64_t kLeast = getenv("LT") ? atoi(getenv("LT")) : 16;
 constexpr int kMaxSplits = 64;  // a lane each in window_join_kernel
 
 Plan plan(const afhip_window_desc& d) {
+  const bool f32 = d.dtype == AFHIP_F32;
   const int64_t group = d.query_heads / d.key_heads, rows = d.queries * group, heads = (int64_t)d.batch * d.key_heads;
   Plan p{};
-  p.step = rows <= 32 || heads * ceil_div(rows, kTileRows) < kFewTiles;
+  // Tiles of 32 rows also where those of 128 are few. Whole calls on MI355X, tiles of 128 / 32, us: f32 over 32
+  // channels 128 tiles 15.9 / 10.1, 256 tiles 17.8 / 32; over 64 40 tiles 28 / 20, 64 tiles 35 / 37; over 128 20 tiles
+  // 39 / 36; f16 over 64 channels 2 tiles 10.5 / 8.9, 128 tiles 12.7 / 16.5; over 128 20 tiles 12.2 / 13.6.
+  const int64_t few = f32 ? (d.head_dim <= 32 ? 256 : 64) : d.head_dim <= 64 ? 64 : 0;
+  p.step = rows <= 32 || heads * ceil_div(rows, kTileRows) < few;
   p.tiles = (int)ceil_div(rows, p.step ? 32 : kTileRows);
+  const int64_t groups = heads * p.tiles;
+  // Eight waves for every CU.
+  p.parts = !p.step && groups < 1024 && !(f32 && d.head_dim > 64) ? 2 : 1;
   // The most keys that a tile's queries see.
   int64_t span = d.keys;
   if (d.left >= 0) {
@@ -429,12 +435,21 @@ Plan plan(const afhip_window_desc& d) {
     const int64_t right = d.right < 0 ? d.keys : d.right;
     span = std::min(span, (int64_t)d.left + right + queries + std::min<int64_t>(d.sinks, d.keys));
   }
-  const int64_t blocks = ceil_div(span, 32), groups = heads * p.tiles;
-  // Eight waves for every CU, each with a few blocks of keys left.
-  p.parts = !p.step && groups < 1024 && !(d.dtype == AFHIP_F32 && d.head_dim > 64) ? 2 : 1;
-  const int64_t wanted = p.step ? kWanted : 512 / p.parts;
-  int64_t splits = std::min(ceil_div(wanted, groups), blocks / kLeast);
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
+  // Into how many parts the keys are split: the shortest of some, by what they take on MI355X in us. A block of 32 keys
+  // takes a workgroup 0.4 (f16, 128 channels; f32 2.6), a workgroup's start and end 4, a CU having one of them at a
+  // time; the keys' bytes come at 5.3 TB/s where all CUs ask for them, at 4 where half do; the join takes 4.5, and its sums go out and in
+  // at 3.5 TB/s.
+  const double block = std::max((f32 ? 2.6 : 0.4) * d.head_dim / 128, 0.15);
+  const double bytes = 2.0 * heads * span * d.head_dim * dtype_size(d.dtype);
+  double best = INFINITY;
+  for (int64_t splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+    const int64_t blocks = ceil_div(span, 32), all = groups * splits;
+    if (splits > 1 && (blocks < 4 * splits || all > 1024)) break;
+    double time = ceil_div(all, p.parts == 2 || p.step ? 256 : 512) * (4 + block * ceil_div(blocks, splits));
+    if (p.step) time = std::max(time, bytes / 5.3e6 * std::pow(std::max(1.0, 256.0 / all), 0.4));
+    if (splits > 1) time += 4.5 + (double)heads * rows * splits * d.head_dim * 8 / 3.5e6;
+    if (time < best) best = time, p.splits = (int)splits;
+  }
   return p;
 }
 

@@ -76,6 +76,7 @@ window_dq_kernel(WindowArgs a) {
   typedef typename Eight<T>::type Frag;
   typedef Tile<T, DP> Tl;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  prefer_one_of_two();
   const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % ROWS, part = wave / ROWS;
   const int heads = a.batch * a.key_heads;
@@ -238,7 +239,6 @@ template <typename T, int DP> struct KeyTile {
   // registers to read fragments ahead of their MFMAs.
   static constexpr bool kShareV = DP == 128 && sizeof(T) == 2;
   static constexpr int kVBytes = kShareV ? kKeys * DP * (int)sizeof(T) : 0, kLds = 2 * kBuffer + kVBytes;
-  static_assert(kLds >= kKeyGroups * DP * 128, "a group's accumulators of one gradient fit");
 };
 
 // Rows that see any key of a tile, and its chunks of them.
@@ -269,14 +269,17 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
   typedef Tile<T, DP> Tl;
   typedef typename Eight<T>::type Frag;
   constexpr int BR = KT::kRows, STEPS = DP / 16, BLOCKS = DP / 32, WAVES = KT::kThreads / 64;
-  constexpr int CHUNKS = Tl::kChunks, STEP = 64 / CHUNKS, COUNT = BR * CHUNKS / 64, UNROLL = sizeof(T) == 2 ? 2 : 1;
+  constexpr int CHUNKS = Tl::kChunks, STEP = 64 / CHUNKS, COUNT = BR * CHUNKS / 64;
   constexpr int TILE = KT::kTileBytes;
+  constexpr float LIFT = sizeof(T) == 2 ? 13.0f : 0.0f;  // on P's exponent, and so on ds
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wave % KT::kKeyGroups, rg = wave / KT::kKeyGroups;
   const int heads = a.batch * a.key_heads;
-  const int pair = blockIdx.x % heads, rest = blockIdx.x / heads, tile = rest / a.chunks, chunk = rest % a.chunks;
+  const int pair = blockIdx.x % heads, rest = blockIdx.x / heads, longs = a.long_tiles * a.chunks;
+  const int tile = rest < longs ? rest / a.chunks : a.long_tiles + (rest - longs) / a.short_chunks;
+  const int chunk = rest < longs ? rest % a.chunks : (rest - longs) % a.short_chunks;
   const int b = pair / a.key_heads, kv = pair % a.key_heads;
   const Sequence s(a, b);
   const int G = a.group, rows = a.queries * G;
@@ -301,26 +304,48 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
     const float per = 1.0f / (float)G;
     const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
     const int chunks = a.head_dim * (int)sizeof(T) / 16;
-    // Of the block to load next: its first row's query and head.
+    // Of the block to load next: its first row's query and head. Where a block holds whole queries every block's rows
+    // lie alike, and their offsets are kept.
     int i0 = begin / G, g0 = begin - i0 * G;
     const int step_i = BR / G, step_g = BR - step_i * G;
+    // Row r of a block is query i0 + t / G, head t % G, with t = r + g0: below 2^17, where the rounded quotient of
+    // t + 1/2 has the right whole part.
+    auto offset = [&](int m, const HeadStrides& s) {
+      const int r = STEP * m + lane / CHUNKS, c = (lane % CHUNKS) ^ Tl::swizzle(r);
+      const int t = r + g0, i = (int)(((float)t + 0.5f) * per), g = t - i * G;
+      return c < chunks ? (uint32_t)i * (uint32_t)s.token + (uint32_t)g * (uint32_t)s.head + 16u * c : kOutOfRange;
+    };
+    constexpr bool KEPT = COUNT % WAVES == 0 && COUNT / WAVES <= 2;
+    uint32_t q_at[KEPT ? COUNT / WAVES : 1], g_at[KEPT ? COUNT / WAVES : 1];
+    if constexpr (KEPT) {
+#pragma unroll
+      for (int j = 0; j < COUNT / WAVES; j++) {
+        q_at[j] = offset(wave + WAVES * j, a.sq);
+        g_at[j] = offset(wave + WAVES * j, a.sdo);
+      }
+    }
     auto issue = [&](int r0, int n) {
-      // Row r0 + r is query i0 + t / G, head t % G, with t = r + g0: below 2^17, where the rounded quotient of
-      // t + 1/2 has the right whole part.
       const int32x4_t qr = make_rsrc(qb + (int64_t)i0 * a.sq.token, 0x7ffffff0u);
       const int32x4_t gr = make_rsrc(gb + (int64_t)i0 * a.sdo.token, 0x7ffffff0u);
       const uint32_t buffer = lds + (uint32_t)(n & 1) * KT::kBuffer;
-#pragma unroll UNROLL
-      for (int j = 0; j < (COUNT + WAVES - 1) / WAVES; j++) {
-        const int m = wave + WAVES * j;
-        if (COUNT % WAVES != 0 && m >= COUNT) break;
-        const int r = STEP * m + lane / CHUNKS, c = (lane % CHUNKS) ^ Tl::swizzle(r);
-        const int t = r + g0, i = (int)(((float)t + 0.5f) * per), g = t - i * G;
-        const bool ok = (c < chunks) & (r0 + r < stop);
-        const uint32_t q_at = (uint32_t)i * (uint32_t)a.sq.token + (uint32_t)g * (uint32_t)a.sq.head + 16u * c;
-        const uint32_t g_at = (uint32_t)i * (uint32_t)a.sdo.token + (uint32_t)g * (uint32_t)a.sdo.head + 16u * c;
-        dma16(qr, buffer + 1024 * m, ok ? q_at : kOutOfRange);
-        dma16(gr, buffer + TILE + 1024 * m, ok ? g_at : kOutOfRange);
+      bool done = false;
+      if constexpr (KEPT) {
+        if (step_g == 0 && r0 + BR <= stop) {
+#pragma unroll
+          for (int j = 0; j < COUNT / WAVES; j++) {
+            dma16(qr, buffer + 1024 * (wave + WAVES * j), q_at[j]);
+            dma16(gr, buffer + TILE + 1024 * (wave + WAVES * j), g_at[j]);
+          }
+          done = true;
+        }
+      }
+      if (!done) {
+#pragma unroll 1
+        for (int m = wave; m < COUNT; m += WAVES) {
+          const bool ok = r0 + STEP * m + lane / CHUNKS < stop;
+          dma16(qr, buffer + 1024 * m, ok ? offset(m, a.sq) : kOutOfRange);
+          dma16(gr, buffer + TILE + 1024 * m, ok ? offset(m, a.sdo) : kOutOfRange);
+        }
       }
       // The rows' statistics, 8 bytes each, 32 rows an instruction: lse and D, and the keys they see. Past the last
       // row zeros, whose rows of dout are zeros too.
@@ -405,7 +430,7 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
         float p[16];
 #pragma unroll
         for (int v = 0; v < 16; v++)
-          p[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -stats[mfma_row(v, lane)].x));
+          p[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, LIFT - stats[mfma_row(v, lane)].x));
         const int2* limits = reinterpret_cast<const int2*>(stats + BR);
         if (partial) {
 #pragma unroll
@@ -425,20 +450,16 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
             y = mma(Tl::nat(gt, sub + col, kk, hi), held(vf[kk]), y);
           }
         }
-        // A probability of 0 stays 0 whatever the gradient is.
         float ds[16];
 #pragma unroll
-        for (int v = 0; v < 16; v++) {
-          const float to = p[v] * (y[v] - stats[mfma_row(v, lane)].y);
-          ds[v] = p[v] == 0.0f ? 0.0f : to;
+        for (int v = 0; v < 16; v++) ds[v] = p[v] * (y[v] - stats[mfma_row(v, lane)].y);
+        if (partial) {  // what is not seen stays 0 whatever its gradient is
+#pragma unroll
+          for (int v = 0; v < 16; v++) ds[v] = p[v] == 0.0f ? 0.0f : ds[v];
         }
         dk.fit(ds);
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-          if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int v = 0; v < 8; v++) p[8 * m + v] *= 0x1p13f;
-          }
           const Frag pf = pack8(p + 8 * m, (Frag*)nullptr), df = pack8(ds + 8 * m, (Frag*)nullptr);
 #pragma unroll
           for (int c = 0; c < BLOCKS; c++) {
@@ -449,65 +470,46 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
       }
     }
   }
-  // The row groups' sums, in their own magnitude, through LDS: one gradient at a time.
-  const float fk = a.scale / dk.scale, fv = sizeof(T) == 2 ? 0x1p-13f : 1.0f;
-#pragma unroll
-  for (int c = 0; c < BLOCKS; c++)
-#pragma unroll
-    for (int v = 0; v < 16; v++) dk.acc[c][v] *= fk, dv[c][v] *= fv;
-  static_assert(KT::kRowGroups == 2, "the second group's sums go to the first");
-  float* shared = reinterpret_cast<float*>(smem) + kg * BLOCKS * 1024 + lane;
-  auto meet = [&](floatx16* x) {
-    block_barrier();
-    if (rg == 1) {
+  // The row groups' sums, in their own magnitude, meet in LDS, one gradient at a time, and leave as whole rows.
+  const float fv = sizeof(T) == 2 ? 0x1p-13f : 1.0f, fk = a.scale * fv / dk.scale;
+  constexpr int PITCH = DP + 4;
+  static_assert(KT::kKeys * PITCH * 4 <= KT::kLds, "a gradient of the tile fits");
+  float* shared = reinterpret_cast<float*>(smem);
+  float* own = shared + (32 * kg + col) * PITCH + 4 * hi;
+  const bool whole = range.chunks <= 1;
+  const int64_t part = ((int64_t)pair * a.tiles + tile) * a.chunks + chunk;
+  auto leave = [&](const floatx16* x, float f, int which) {
+    for (int group = KT::kRowGroups - 1; group >= 0; group--) {
+      block_barrier();
+      if (rg != group) continue;
 #pragma unroll
       for (int c = 0; c < BLOCKS; c++)
 #pragma unroll
-        for (int v = 0; v < 16; v++) shared[(16 * c + v) * 64] = x[c][v];
+        for (int g = 0; g < 4; g++) {
+          floatx4* at = reinterpret_cast<floatx4*>(own + 32 * c + 8 * g);
+          floatx4 y{x[c][4 * g] * f, x[c][4 * g + 1] * f, x[c][4 * g + 2] * f, x[c][4 * g + 3] * f};
+          if (group < KT::kRowGroups - 1) y += *at;
+          *at = y;
+        }
     }
     block_barrier();
-    if (rg == 0) {
-#pragma unroll
-      for (int c = 0; c < BLOCKS; c++)
-#pragma unroll
-        for (int v = 0; v < 16; v++) x[c][v] += shared[(16 * c + v) * 64];
+    const int quads = a.head_dim / 4;
+    for (int n = threadIdx.x; n < KT::kKeys * quads; n += KT::kThreads) {
+      const int j = n / quads, ch = 4 * (n % quads);
+      if (j0 + j >= a.keys) break;
+      floatx4 y = *reinterpret_cast<const floatx4*>(shared + j * PITCH + ch);
+      if (!whole) {
+        *reinterpret_cast<floatx4*>(a.partial + ((2 * part + which) * KT::kKeys + j) * a.head_dim + ch) = y;
+      } else {
+        if (j0 + j >= s.keys) y = floatx4{};
+        T* to = reinterpret_cast<T*>(which ? a.dv : a.dk) +
+                (((int64_t)b * a.keys + j0 + j) * a.key_heads + kv) * a.head_dim + ch;
+        put4(to, y[0], y[1], y[2], y[3]);
+      }
     }
   };
-  meet(dk.acc);
-  meet(dv);
-  if (rg == 1 || key >= a.keys) return;
-  if (range.chunks > 1) {
-    const int64_t part = ((int64_t)pair * a.tiles + tile) * a.chunks + chunk;
-    float* to = a.partial + (part * 2 * KT::kKeys + 32 * kg + col) * a.head_dim;
-#pragma unroll
-    for (int c = 0; c < BLOCKS; c++)
-#pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const int ch = 32 * c + 8 * g + 4 * hi;
-        if (ch >= a.head_dim) continue;
-#pragma unroll
-        for (int which = 0; which < 2; which++) {
-          const floatx16& x = which ? dv[c] : dk.acc[c];
-          *reinterpret_cast<floatx4*>(to + which * KT::kKeys * a.head_dim + ch) =
-              floatx4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
-        }
-      }
-    return;
-  }
-  const int64_t at = (((int64_t)b * a.keys + key) * a.key_heads + kv) * a.head_dim;
-  T *tk = reinterpret_cast<T*>(a.dk) + at, *tv = reinterpret_cast<T*>(a.dv) + at;
-#pragma unroll
-  for (int c = 0; c < BLOCKS; c++)
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const int ch = 32 * c + 8 * g + 4 * hi;
-      if (ch >= a.head_dim) continue;
-      const floatx16 &x = dk.acc[c], &y = dv[c];
-      put4(tk + ch, live ? x[4 * g] : 0.0f, live ? x[4 * g + 1] : 0.0f, live ? x[4 * g + 2] : 0.0f,
-           live ? x[4 * g + 3] : 0.0f);
-      put4(tv + ch, live ? y[4 * g] : 0.0f, live ? y[4 * g + 1] : 0.0f, live ? y[4 * g + 2] : 0.0f,
-           live ? y[4 * g + 3] : 0.0f);
-    }
+  leave(dk.acc, fk, 0);
+  leave(dv, fv, 1);
 }
 
 // Adds up the chunks of the tiles that have several, in order: 1,024 values a workgroup.
@@ -533,7 +535,11 @@ template <typename T> __global__ __launch_bounds__(256) void window_dkv_join_ker
 
 // The key tiles, and the rows of a chunk.
 struct KeyPlan {
-  int tile_keys, tiles, chunks, chunk_rows;
+  int tile_keys, tiles, chunk_rows;
+  int long_tiles, chunks, short_chunks;  // tiles that every row may see, the chunks of one, those of the others
+  int64_t groups(int64_t heads) const {
+    return heads * ((int64_t)long_tiles * chunks + (int64_t)(tiles - long_tiles) * short_chunks);
+  }
 };
 
 KeyPlan key_plan(const afhip_window_desc& d) {
@@ -546,11 +552,15 @@ KeyPlan key_plan(const afhip_window_desc& d) {
   const int64_t span = d.left < 0 || d.right < 0
                            ? all : std::min<int64_t>(all, ((int64_t)d.left + d.right + p.tile_keys) * group);
   const int64_t most = d.left < 0 || d.sinks > 0 ? all : span, groups = (int64_t)d.batch * d.key_heads * p.tiles;
-  // Two workgroups for each CU, of some blocks of rows.
-  int64_t rows = std::max<int64_t>(ceil_div(span * groups, 512), 128);
+  p.long_tiles = d.left < 0 ? p.tiles : (int)std::min<int64_t>(p.tiles, ceil_div(d.sinks, p.tile_keys));
+  // Chunks that make about 400 workgroups: with one a CU, fewer leave CUs idle at the end, more cost each a start and
+  // sums to join. 4,096 tokens, 16 heads over 4, window 1,024, dk and dv with the join in us on MI355X: 256 workgroups
+  // 154, 300 150, 350 139, 400 134, 512 159, 600 146, 800 156, 1,000 191.
+  int64_t rows = std::max<int64_t>(ceil_div(span * groups, 400), 128);
   rows = std::max(rows, ceil_div(most, 64));
   p.chunk_rows = (int)round_up(rows, 64);
   p.chunks = (int)ceil_div(most, p.chunk_rows);
+  p.short_chunks = (int)ceil_div(span, p.chunk_rows);
   return p;
 }
 
@@ -586,14 +596,17 @@ template <typename T, int DP> int launch_backward(WindowArgs& a, const KeyPlan& 
   const int64_t heads = (int64_t)a.batch * a.key_heads, rows = (int64_t)a.queries * a.group;
   AFHIP_REQUIRE(p.tile_keys == KT::kKeys, "key tiles of %d keys, not %d", KT::kKeys, p.tile_keys);
   const int parts = (int)ceil_div(2 * KT::kKeys * a.head_dim, 1024);
-  AFHIP_REQUIRE(heads * p.tiles * std::max(p.chunks, parts) < ((int64_t)1 << 31), "attention grid too large");
+  AFHIP_REQUIRE(p.groups(heads) < ((int64_t)1 << 31) && heads * p.tiles * parts < ((int64_t)1 << 31),
+                "attention grid too large");
   if ((s = launch_dq_any<T, DP>(a, heads, rows, st))) return s;
   a.tiles = p.tiles;
   a.chunks = p.chunks;
   a.chunk_rows = p.chunk_rows;
+  a.long_tiles = p.long_tiles;
+  a.short_chunks = p.short_chunks;
   auto kkv = window_dkv_kernel<T, DP>;
   if ((s = allow_lds((const void*)kkv, KT::kLds))) return s;
-  if ((s = launch("window.dkv", kkv, dim3((unsigned)(heads * p.tiles * p.chunks)), dim3(KT::kThreads), KT::kLds, st, a)))
+  if ((s = launch("window.dkv", kkv, dim3((unsigned)p.groups(heads)), dim3(KT::kThreads), KT::kLds, st, a)))
     return s;
   if (p.chunks == 1) return AFHIP_OK;
   return launch("window.dkv_join", window_dkv_join_kernel<T>, dim3((unsigned)(heads * p.tiles * parts)), dim3(256), 0, st,
