@@ -58,23 +58,31 @@ def address(tensor):
     return None if tensor is None else tensor.data_ptr()
 
 
-def _stream_getter():
-    """torch's current stream of a device as a hipStream_t. The direct getter where this torch has it: the public way
-    makes a Stream object first, which takes as long as the launch of a small kernel (2.7 us of 0.07)."""
+def _direct(name: str, otherwise):
+    """A getter of torch's own bindings where this torch has it, else the public one, which makes objects on the way
+    (the current stream 2.7 us in place of 0.07, as long as the launch of a small kernel)."""
     import torch
 
-    direct = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return direct or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    return getattr(torch._C, name, None) or otherwise(torch)
 
 
-_stream = None
+_stream = _device = None
 
 
 def current_stream(index: int) -> int:
+    """torch's current stream of a device, as a hipStream_t."""
     global _stream
     if _stream is None:
-        _stream = _stream_getter()
+        _stream = _direct("_cuda_getCurrentRawStream",
+                          lambda torch: lambda i: torch.cuda.current_stream(i).cuda_stream)
     return _stream(index)
+
+
+def current_device() -> int:
+    global _device
+    if _device is None:
+        _device = _direct("_cuda_getDevice", lambda torch: torch.cuda.current_device)
+    return _device()
 
 
 def packed_like(tensor):

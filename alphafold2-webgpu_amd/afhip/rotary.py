@@ -14,7 +14,8 @@ import numpy as np
 
 from . import _lib
 from .device import device, open_device
-from .heads import FORMS, address, check_device, check_heads, check_ints, current_stream, form, packed_like, strides
+from .heads import (FORMS, address, check_device, check_heads, check_ints, current_device, current_stream, form,
+                    packed_like, strides)
 
 _DT = {"f32": _lib.F32, "f16": _lib.F16}
 _LAYOUTS = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
@@ -150,7 +151,7 @@ class HeadRotary:
         into a cache. q_out may be q, and k_out k."""
         import torch
 
-        if _current_device() != self._device:
+        if current_device() != self._device:
             with torch.cuda.device(self._device):
                 return self(q, k, v, past=past, lengths=lengths, positions=positions, q_out=q_out, k_out=k_out,
                             k_cache=k_cache, v_cache=v_cache)
@@ -206,7 +207,7 @@ class HeadRotary:
         "dkey_scale", with "layer" "dquery_offset" and "dkey_offset" too (f32 [head_dim])."""
         import torch
 
-        if _current_device() != self._device:
+        if current_device() != self._device:
             with torch.cuda.device(self._device):
                 return self.backward(q, k, dq_out, dk_out, past=past, lengths=lengths, positions=positions)
         self._ready()

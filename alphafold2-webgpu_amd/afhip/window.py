@@ -14,7 +14,8 @@ import math
 
 from . import _lib
 from .device import device, open_device
-from .heads import FORMS, address, check_device, check_heads, check_ints, current_stream, form, packed_like, strides
+from .heads import (FORMS, address, check_device, check_heads, check_ints, current_device, current_stream, form,
+                    packed_like, strides)
 
 _DT = {"f32": _lib.F32, "f16": _lib.F16}
 
@@ -76,7 +77,7 @@ class WindowAttention:
         read."""
         import torch
 
-        if _current_device() != self._device:
+        if current_device() != self._device:
             with torch.cuda.device(self._device):
                 return self(q, k, v, query_lengths=query_lengths, key_lengths=key_lengths, out=out,
                             return_lse=return_lse)
@@ -106,7 +107,7 @@ class WindowAttention:
         the query heads that read them. Zeros past the lengths. The same bits at every call."""
         import torch
 
-        if _current_device() != self._device:
+        if current_device() != self._device:
             with torch.cuda.device(self._device):
                 return self.backward(q, k, v, out, lse, dout, query_lengths=query_lengths, key_lengths=key_lengths)
         key = ("backward", form(q), form(k), form(v), form(out), form(lse), form(dout), form(query_lengths),

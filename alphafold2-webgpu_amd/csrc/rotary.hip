@@ -150,32 +150,61 @@ template <typename T, int LANES, int NORM> __global__ __launch_bounds__(kThreads
   const int count = min(s.tile_tokens, a.tokens - first);
   const int unit = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int D = a.head_dim, pairs = a.rotary_dim / 2, heads = s.heads;
+  const char* from = s.x + b * s.sx.batch + first * s.sx.token;
+  const int token = (int)s.sx.token;  // at most 2^24, of at most 16 tokens
+  const int total = count * heads;
+  const bool active = 8 * unit < D, turned = 8 * unit < a.rotary_dim, half = a.layout == AFHIP_ROTARY_HALF;
+  const int c0 = turned && half ? 4 * unit : 8 * unit, c1 = turned && half ? pairs + 4 * unit : 8 * unit + 4;
+  // A token past the length is read all the same, and not used. The first rows are on their way before all else.
+  float x[kInFlight][8];
+  auto load = [&](int n0) {
+#pragma unroll
+    for (int r = 0; r < kInFlight; r++) {
+      const int n = min(n0 + r * GROUPS, total - 1), t = n / heads, h = n % heads;
+      if (!active) continue;
+      const char* p = from + t * token + h * s.sx.head;
+      load4<T>(p, c0, x[r]);
+      load4<T>(p, c1, x[r] + 4);
+    }
+  };
+  if (!active) {
+#pragma unroll
+    for (int r = 0; r < kInFlight; r++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[r][j] = 0.0f;
+  }
+  if (which != 2) load(group);
   const int live = live_tokens(a, b);
   const int64_t past = a.past ? a.past[b] : 0;
-  const char* from = s.x + b * s.sx.batch + first * s.sx.token;
-  // Row of `out` that the tile's first token goes to; only those in [0, rows)
-  // of a cache are written.
+  // Row of `out` that the tile's first token goes to; only those in [0, rows) of a cache are written.
   const int64_t row0 = s.rows ? past + first : first;
   char* to = s.out + b * s.so.batch + row0 * s.so.token;
-  const int total = count * heads;
   auto writes = [&](int t) {
     return s.rows == 0 || (first + t < live && row0 + t >= 0 && row0 + t < s.rows);
   };
   if (which == 2) {  // the values, bit for bit
     constexpr int PARTS = 8 * (int)sizeof(T) / 16;
-    if (8 * unit >= D) return;
-    for (int n = group; n < total; n += GROUPS) {
-      const int t = n / heads, h = n % heads;
-      if (!writes(t)) continue;
-      const u32x4* p = reinterpret_cast<const u32x4*>(from + t * s.sx.token + h * s.sx.head);
-      u32x4* o = reinterpret_cast<u32x4*>(to + t * s.so.token + h * s.so.head);
+    if (!active) return;
+    for (int n0 = group; n0 < total; n0 += kInFlight * GROUPS) {
+      u32x4 v[kInFlight][PARTS];
 #pragma unroll
-      for (int j = 0; j < PARTS; j++) o[PARTS * unit + j] = p[PARTS * unit + j];
+      for (int r = 0; r < kInFlight; r++) {
+        const int n = min(n0 + r * GROUPS, total - 1);
+        const u32x4* p = reinterpret_cast<const u32x4*>(from + n / heads * token + n % heads * s.sx.head);
+#pragma unroll
+        for (int j = 0; j < PARTS; j++) v[r][j] = p[PARTS * unit + j];
+      }
+#pragma unroll
+      for (int r = 0; r < kInFlight; r++) {
+        const int n = n0 + r * GROUPS, t = n / heads, h = n % heads;
+        if (n >= total || !writes(t)) continue;
+        u32x4* o = reinterpret_cast<u32x4*>(to + t * s.so.token + h * s.so.head);
+#pragma unroll
+        for (int j = 0; j < PARTS; j++) o[PARTS * unit + j] = v[r][j];
+      }
     }
     return;
   }
-  const bool active = 8 * unit < D, turned = 8 * unit < a.rotary_dim, half = a.layout == AFHIP_ROTARY_HALF;
-  const int c0 = turned && half ? 4 * unit : 8 * unit, c1 = turned && half ? pairs + 4 * unit : 8 * unit + 4;
   float w[8], c[8];
   if (NORM != AFHIP_HEAD_NORM_NONE && active) {
     load4<float>(reinterpret_cast<const char*>(s.scale), c0, w);
@@ -187,38 +216,29 @@ template <typename T, int LANES, int NORM> __global__ __launch_bounds__(kThreads
   }
   fill_turns(a, b, first, count, turns);
   __syncthreads();
-  for (int n0 = group; n0 < total; n0 += kInFlight * GROUPS) {
-    float x[kInFlight][8];
-#pragma unroll
-    for (int r = 0; r < kInFlight; r++) {
-      const int n = n0 + r * GROUPS, t = n / heads, h = n % heads;
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[r][j] = 0.0f;
-      if (n >= total || first + t >= live || !active) continue;
-      const char* p = from + t * s.sx.token + h * s.sx.head;
-      load4<T>(p, c0, x[r]);
-      load4<T>(p, c1, x[r] + 4);
-    }
+  for (int n0 = group; n0 < total;) {
 #pragma unroll
     for (int r = 0; r < kInFlight; r++) {
       const int n = n0 + r * GROUPS, t = n / heads, h = n % heads;
       if (n >= total) break;
-      if (first + t < live) {
-        if constexpr (NORM != AFHIP_HEAD_NORM_NONE) {
-          normalize<LANES, NORM>(x[r], active, D, a.epsilon);
+      if constexpr (NORM != AFHIP_HEAD_NORM_NONE) {
+        normalize<LANES, NORM>(x[r], active, D, a.epsilon);
 #pragma unroll
-          for (int j = 0; j < 8; j++) {
-            x[r][j] *= w[j];
-            if (NORM == AFHIP_HEAD_NORM_LAYER) x[r][j] += c[j];
-          }
+        for (int j = 0; j < 8; j++) {
+          x[r][j] *= w[j];
+          if (NORM == AFHIP_HEAD_NORM_LAYER) x[r][j] += c[j];
         }
-        if (turned) turn4<1>(turns + t * pairs + 4 * unit, half, x[r]);
       }
+      if (turned) turn4<1>(turns + t * pairs + 4 * unit, half, x[r]);
       if (!active || !writes(t)) continue;
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[r][j] = first + t < live ? x[r][j] : 0.0f;
       char* p = to + t * s.so.token + h * s.so.head;
       store4<T>(p, c0, x[r]);
       store4<T>(p, c1, x[r] + 4);
     }
+    n0 += kInFlight * GROUPS;
+    if (n0 < total) load(n0);
   }
 }
 
@@ -376,7 +396,7 @@ int check(const afhip_rotary_desc* desc) {
 
 // What both ways have, and the sides' strides.
 RotaryArgs fill(const afhip_rotary_desc& d, const int32_t* past, const int32_t* lengths, const int32_t* positions,
-                const double* frequencies, const float* query_scale, const float* key_scale) {
+                const double* frequencies, const float* query_scale, const float* key_scale, int least) {
   RotaryArgs a{};
   const int kt = d.capacity ? d.capacity : d.tokens;
   a.side[0].sx = head_strides(d.q, d.tokens, d.query_heads, d.head_dim, d.dtype);
@@ -402,12 +422,14 @@ RotaryArgs fill(const afhip_rotary_desc& d, const int32_t* past, const int32_t* 
   a.epsilon = d.epsilon;
   a.turn = d.rotation_scale;
   // As many tokens at once as make kRowsWanted rows, fewer where that leaves
-  // workgroups few.
+  // workgroups few: `least` of them are aimed at. 3 sequences of 1,021
+  // tokens, 8 + 8 heads of 32, f32, take 7.4 us at 512 and 9.1 at 1024; back,
+  // 4,096 tokens of 32 + 8 heads of 128, f16, take 36.7 at 512 and 34.9 at 1024.
   for (Side& s : a.side) {
     const int64_t tokens = (int64_t)d.batch * d.tokens;
     int64_t n = ceil_div(kRowsWanted, s.heads);
     if (n > kMostTokens) n = kMostTokens;
-    if (n > tokens / 1024) n = tokens / 1024 > 1 ? tokens / 1024 : 1;
+    if (n > tokens / least) n = tokens / least > 1 ? tokens / least : 1;
     s.tile_tokens = (int)n;
     s.tiles = (int)ceil_div(d.tokens, n);
     s.groups = d.batch * s.tiles;
@@ -480,7 +502,7 @@ int afhip_rotary_run(const afhip_rotary_desc* desc, const void* q, const void* k
   const float* scales[] = {query_scale, key_scale};
   const float* offsets[] = {query_offset, key_offset};
   if ((s = check_vectors(d, frequencies, scales, offsets))) return s;
-  RotaryArgs a = fill(d, past, lengths, positions, frequencies, query_scale, key_scale);
+  RotaryArgs a = fill(d, past, lengths, positions, frequencies, query_scale, key_scale, 512);
   const int kt = d.capacity ? d.capacity : d.tokens;
   if ((s = check_address("q", q)) || (s = check_address("k", k)) ||
       (s = check_side("q_out", a.side[0].so, q_out, d.tokens, d.query_heads, d, true)) ||
@@ -522,7 +544,7 @@ int afhip_rotary_backward(const afhip_rotary_desc* desc, const void* q, const vo
   AFHIP_REQUIRE(d.capacity == 0, "the way back takes no cache");
   const float* scales[] = {query_scale, key_scale};
   if ((s = check_vectors(d, frequencies, scales, nullptr))) return s;
-  RotaryArgs a = fill(d, past, lengths, positions, frequencies, query_scale, key_scale);
+  RotaryArgs a = fill(d, past, lengths, positions, frequencies, query_scale, key_scale, 1024);
   // The descriptor's q_out and k_out are the gradients' strides; dq and dk are packed.
   for (int i = 0; i < 2; i++) a.side[i].sg = a.side[i].so;
   if ((s = check_address("q", q)) || (s = check_address("k", k)) ||

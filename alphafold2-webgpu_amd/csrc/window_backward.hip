@@ -410,7 +410,7 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
     // Rows that see all of them.
     const int never = rows + 1;
     const int full_begin =
-        wj0 + 32 > s.keys ? never : a.right < 0 ? 0 : min(rows, max(0, wj0 + 31 - a.right - s.offset) * G);
+        wj0 + 32 > s.keys ? never : a.right < 0 ? 0 : min(s.queries, max(0, wj0 + 31 - a.right - s.offset)) * G;
     const int full_stop =
         a.left < 0 || wj0 + 32 <= a.sinks ? never : min(s.queries, max(0, wj0 + a.left - s.offset + 1)) * G;
 #pragma unroll 1
