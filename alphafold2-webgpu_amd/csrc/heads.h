@@ -55,4 +55,11 @@ inline int check_address(const char* name, const void* p) {
   return AFHIP_OK;
 }
 
+// A launch has fewer than 2^32 threads.
+inline int check_grid(int64_t groups, int threads) {
+  AFHIP_REQUIRE(groups * threads < ((int64_t)1 << 32), "%lld workgroups of %d threads are too many for one launch",
+                (long long)groups, threads);
+  return AFHIP_OK;
+}
+
 }  // namespace afhip

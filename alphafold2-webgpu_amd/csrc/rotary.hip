@@ -438,7 +438,9 @@ RotaryArgs fill(const afhip_rotary_desc& d, const int32_t* past, const int32_t* 
 }
 
 template <typename T, int LANES, int NORM> int launch_way(const RotaryArgs& a, bool back, hipStream_t st) {
-  const dim3 grid((unsigned)(a.side[0].groups + a.side[1].groups + a.side[2].groups));
+  const int64_t groups = (int64_t)a.side[0].groups + a.side[1].groups + a.side[2].groups;
+  if (int s = check_grid(groups, kThreads)) return s;
+  const dim3 grid((unsigned)groups);
   if (back)
     return launch("rotary.backward", rotary_backward_kernel<T, LANES, NORM>, grid, dim3(kThreads), 0, st, a);
   return launch("rotary", rotary_kernel<T, LANES, NORM>, grid, dim3(kThreads), 0, st, a);

@@ -16,7 +16,8 @@ struct WindowArgs {
   char* out;
   float* lse;
   const int32_t *query_lengths, *key_lengths;
-  // Split keys: [row][split] of head_dim sums, the reference point, the total. The way back: [tile][chunk] of dk and dv.
+  // Split keys: [row][split] of head_dim sums, the reference point, the total. The way back: dk and dv of each chunk
+  // of the tiles that may have several.
   float* partial;
   HeadStrides sq, sk, sv, so;
   int batch, queries, keys, query_heads, key_heads, group, head_dim;
@@ -33,6 +34,7 @@ struct WindowArgs {
   // dk and dv: the most chunks of rows that a tile of keys has, the rows of one; tiles that all rows may see, and the
   // chunks of the others.
   int chunks, chunk_rows, long_tiles, short_chunks;
+  int parts;  // chunks of a key head that leave partial sums
 };
 
 typedef float floatx8 __attribute__((ext_vector_type(8)));

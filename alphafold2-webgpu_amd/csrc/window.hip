@@ -1,7 +1,8 @@
 // Attention over a window of keys and the first few ("sinks"), for prompts and
 // for single tokens against a cache:
 //
-//   p = key_length - query_length + i;  key j is seen iff j < key_length, j <= p + right, and j >= p - left or j < sinks
+//   p = key_length - query_length + i;  key j is seen iff j < key_length, j <= p + right, and j >= p - left or
+//   j < sinks
 //   out = sum_j e^(s_j - m) v_j / l,  l = sum_j e^(s_j - m),  lse = m + ln l,  s_j = scale q . k_j
 //
 // in one pass over the keys with a running reference point m. Query heads that
@@ -13,7 +14,7 @@
 // the reference point and the sum stay inside the lane (and the lane 32 away),
 // and the probabilities feed the second product from the registers they were
 // computed in. K and V go to LDS by DMA; V^T comes from gfx950's transposing LDS
-// read. f32 runs the same on the f32 MFMA.
+// read. f32 runs the same, its values as three bf16 each.
 //
 // Blocks of keys that no query of a workgroup sees are not visited, rows of one
 // that none sees are loaded as zeros (whatever is there, infinities and NaN too),
@@ -280,7 +281,8 @@ __global__ __launch_bounds__((kStepThreads<T, DP>)) void window_step_kernel(Wind
   const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = a.batch * a.key_heads;
-  const int pair = blockIdx.x % heads, rest = blockIdx.x / heads, tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
+  const int pair = blockIdx.x % heads, rest = blockIdx.x / heads;
+  const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
   const int b = pair / a.key_heads, kv = pair % a.key_heads;
   const Sequence s(a, b);
   const int all = a.queries * a.group, r0 = 32 * tile, rows = min(32, all - r0);
@@ -437,8 +439,8 @@ Plan plan(const afhip_window_desc& d) {
   }
   // Into how many parts the keys are split: the shortest of some, by what they take on MI355X in us. A block of 32 keys
   // takes a workgroup 0.4 (f16, 128 channels; f32 2.6), a workgroup's start and end 4, a CU having one of them at a
-  // time; the keys' bytes come at 5.3 TB/s where all CUs ask for them, at 4 where half do; the join takes 4.5, and its sums go out and in
-  // at 3.5 TB/s.
+  // time; the keys' bytes come at 5.3 TB/s where all CUs ask for them, at 4 where half do; the join takes 4.5, and its
+  // sums go out and in at 3.5 TB/s.
   const double block = std::max((f32 ? 2.6 : 0.4) * d.head_dim / 128, 0.15);
   const double bytes = 2.0 * heads * span * d.head_dim * dtype_size(d.dtype);
   double best = INFINITY;
@@ -462,18 +464,18 @@ template <typename T, int DP, int PARTS>
 int launch_rows(const WindowArgs& a, const Plan& p, int64_t groups, hipStream_t st) {
   constexpr size_t lds = kRowsLds<T, DP, PARTS>;
   auto k = p.splits > 1 ? window_rows_kernel<T, DP, true, PARTS> : window_rows_kernel<T, DP, false, PARTS>;
-  if (int s = allow_lds((const void*)k, lds)) return s;
+  int s;
+  if ((s = check_grid(groups, 64 * kWaves * PARTS)) || (s = allow_lds((const void*)k, lds))) return s;
   return launch("window.rows", k, dim3((unsigned)groups), dim3(64 * kWaves * PARTS), lds, st, a);
 }
 
 template <typename T, int DP> int launch_forward(const WindowArgs& a, const Plan& p, hipStream_t st) {
   int s;
   const int64_t groups = (int64_t)a.batch * a.key_heads * p.tiles * p.splits;
-  AFHIP_REQUIRE(groups < ((int64_t)1 << 31), "attention grid too large");
   if (p.step) {
     typedef Step<T, DP> S;
     auto k = window_step_kernel<T, DP>;
-    if ((s = allow_lds((const void*)k, S::kLds))) return s;
+    if ((s = check_grid(groups, 64 * S::kWaves)) || (s = allow_lds((const void*)k, S::kLds))) return s;
     s = launch("window.step", k, dim3((unsigned)groups), dim3(64 * S::kWaves), S::kLds, st, a);
   } else {
     s = p.parts == 2 ? launch_rows<T, DP, kTwoParts<T, DP> ? 2 : 1>(a, p, groups, st)
@@ -481,7 +483,7 @@ template <typename T, int DP> int launch_forward(const WindowArgs& a, const Plan
   }
   if (s || p.splits == 1) return s;
   const int64_t rows = (int64_t)a.batch * a.queries * a.query_heads;
-  AFHIP_REQUIRE(ceil_div(rows, 4) < ((int64_t)1 << 31), "attention grid too large");
+  if ((s = check_grid(ceil_div(rows, 4), 256))) return s;
   return launch("window.join", window_join_kernel<T>, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a);
 }
 

@@ -68,8 +68,9 @@ template <typename T, int DP, int ROWS, int PARTS, int WK> struct RowTile {
 };
 
 template <typename T, int DP, int ROWS, int PARTS, int WK>
-__global__ __launch_bounds__((RowTile<T, DP, ROWS, PARTS, WK>::kThreads), (RowTile<T, DP, ROWS, PARTS, WK>::kGroups)) void
-window_dq_kernel(WindowArgs a) {
+__global__
+__launch_bounds__((RowTile<T, DP, ROWS, PARTS, WK>::kThreads), (RowTile<T, DP, ROWS, PARTS, WK>::kGroups))
+void window_dq_kernel(WindowArgs a) {
   constexpr int BK = WK * PARTS, STEPS = DP / 16, BLOCKS = DP / 32;
   constexpr int HELD = RowTile<T, DP, ROWS, PARTS, WK>::kRows;
   typedef TileLoad<T, DP, BK, ROWS * PARTS> Load;
@@ -366,8 +367,8 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
       load.issue(a.v + b * a.sv.batch + kv * a.sv.head, a.sv.token, j0, lds + 2 * KT::kBuffer, wave, false,
                  [&](int key) { return key < s.keys; });
     }
-    // Over 128 channels of f32 K and V are held as they are, and made three bf16 at each use, which costs a tenth of the
-    // MFMAs' time: as parts they would not fit.
+    // Over 128 channels of f32 K and V are held as they are, and made three bf16 at each use, which costs a tenth of
+    // the MFMAs' time: as parts they would not fit.
     constexpr bool RAW = sizeof(T) == 4 && DP == 128;
     typedef typename std::conditional<RAW, floatx8, Frag>::type Held;
     Held kf[STEPS], vf[KT::kShareV ? 1 : STEPS];
@@ -477,7 +478,7 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
   float* shared = reinterpret_cast<float*>(smem);
   float* own = shared + (32 * kg + col) * PITCH + 4 * hi;
   const bool whole = range.chunks <= 1;
-  const int64_t part = ((int64_t)pair * a.tiles + tile) * a.chunks + chunk;
+  const int64_t part = (int64_t)pair * a.parts + rest;
   auto leave = [&](const floatx16* x, float f, int which) {
     for (int group = KT::kRowGroups - 1; group >= 0; group--) {
       block_barrier();
@@ -513,7 +514,8 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
 }
 
 // Adds up the chunks of the tiles that have several, in order: 1,024 values a workgroup.
-template <typename T> __global__ __launch_bounds__(256) void window_dkv_join_kernel(WindowArgs a, int tile_keys, int parts) {
+template <typename T>
+__global__ __launch_bounds__(256) void window_dkv_join_kernel(WindowArgs a, int tile_keys, int parts) {
   const int heads = a.batch * a.key_heads;
   const int pair = blockIdx.x % heads, rest = blockIdx.x / heads, tile = rest / parts, part = rest % parts;
   const int b = pair / a.key_heads, kv = pair % a.key_heads, D = a.head_dim;
@@ -524,7 +526,9 @@ template <typename T> __global__ __launch_bounds__(256) void window_dkv_join_ker
   if (n >= size) return;
   const int which = n >= tile_keys * D, m = n - which * tile_keys * D, key = tile * tile_keys + m / D, ch = m % D;
   if (key >= a.keys) return;
-  const float* from = a.partial + ((int64_t)pair * a.tiles + tile) * a.chunks * size + n;
+  const int first = tile < a.long_tiles ? tile * a.chunks
+                                        : a.long_tiles * a.chunks + (tile - a.long_tiles) * a.short_chunks;
+  const float* from = a.partial + ((int64_t)pair * a.parts + first) * size + n;
   floatx4 x{};
 #pragma unroll 4
   for (int c = 0; c < range.chunks; c++) x += *reinterpret_cast<const floatx4*>(from + (int64_t)c * size);
@@ -539,6 +543,11 @@ struct KeyPlan {
   int long_tiles, chunks, short_chunks;  // tiles that every row may see, the chunks of one, those of the others
   int64_t groups(int64_t heads) const {
     return heads * ((int64_t)long_tiles * chunks + (int64_t)(tiles - long_tiles) * short_chunks);
+  }
+  // Tiles, of the first, that may have several chunks, and those chunks.
+  int joined() const { return chunks == 1 ? 0 : short_chunks == 1 ? long_tiles : tiles; }
+  int64_t parts() const {
+    return joined() == tiles ? groups(1) : (int64_t)joined() * chunks;
   }
 };
 
@@ -565,17 +574,16 @@ KeyPlan key_plan(const afhip_window_desc& d) {
 }
 
 size_t chunk_bytes(const afhip_window_desc& d, const KeyPlan& p) {
-  if (p.chunks == 1) return 0;
-  return (size_t)d.batch * d.key_heads * p.tiles * p.chunks * 2 * p.tile_keys * d.head_dim * sizeof(float);
+  return (size_t)d.batch * d.key_heads * p.parts() * 2 * p.tile_keys * d.head_dim * sizeof(float);
 }
 
 template <typename T, int DP, int ROWS, int PARTS, int WK>
 int launch_dq(WindowArgs& a, int64_t heads, int64_t rows, hipStream_t st) {
   typedef RowTile<T, DP, ROWS, PARTS, WK> RT;
   a.tiles = (int)ceil_div(rows, RT::kRows);
-  AFHIP_REQUIRE(heads * a.tiles < ((int64_t)1 << 31), "attention grid too large");
   auto k = window_dq_kernel<T, DP, ROWS, PARTS, WK>;
-  if (int s = allow_lds((const void*)k, RT::kLds)) return s;
+  int s;
+  if ((s = check_grid(heads * a.tiles, RT::kThreads)) || (s = allow_lds((const void*)k, RT::kLds))) return s;
   return launch("window.dq", k, dim3((unsigned)(heads * a.tiles)), dim3(RT::kThreads), RT::kLds, st, a);
 }
 
@@ -596,21 +604,20 @@ template <typename T, int DP> int launch_backward(WindowArgs& a, const KeyPlan& 
   const int64_t heads = (int64_t)a.batch * a.key_heads, rows = (int64_t)a.queries * a.group;
   AFHIP_REQUIRE(p.tile_keys == KT::kKeys, "key tiles of %d keys, not %d", KT::kKeys, p.tile_keys);
   const int parts = (int)ceil_div(2 * KT::kKeys * a.head_dim, 1024);
-  AFHIP_REQUIRE(p.groups(heads) < ((int64_t)1 << 31) && heads * p.tiles * parts < ((int64_t)1 << 31),
-                "attention grid too large");
+  if ((s = check_grid(p.groups(heads), KT::kThreads)) || (s = check_grid(heads * p.joined() * parts, 256))) return s;
   if ((s = launch_dq_any<T, DP>(a, heads, rows, st))) return s;
   a.tiles = p.tiles;
   a.chunks = p.chunks;
   a.chunk_rows = p.chunk_rows;
   a.long_tiles = p.long_tiles;
   a.short_chunks = p.short_chunks;
+  a.parts = (int)p.parts();
   auto kkv = window_dkv_kernel<T, DP>;
   if ((s = allow_lds((const void*)kkv, KT::kLds))) return s;
   if ((s = launch("window.dkv", kkv, dim3((unsigned)p.groups(heads)), dim3(KT::kThreads), KT::kLds, st, a)))
     return s;
-  if (p.chunks == 1) return AFHIP_OK;
-  return launch("window.dkv_join", window_dkv_join_kernel<T>, dim3((unsigned)(heads * p.tiles * parts)), dim3(256), 0, st,
-                a, KT::kKeys, parts);
+  return launch("window.dkv_join", window_dkv_join_kernel<T>, dim3((unsigned)(heads * p.joined() * parts)), dim3(256),
+                0, st, a, KT::kKeys, parts);
 }
 
 template <typename T> int launch_width(WindowArgs& a, const KeyPlan& p, hipStream_t st) {

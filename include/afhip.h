@@ -472,7 +472,9 @@ AFHIP_API int afhip_attention_run(const afhip_attention_desc* desc, const void* 
 /* Where an element of a tensor [batch][tokens][heads][channels] lies, in
  * elements; channels are contiguous. token 0: packed, in that order. A batch
  * or head stride of 0 repeats one entry (inputs only). Strides that are used
- * are multiples of 16 bytes, and so are all tensors' addresses. No counterpart
+ * are multiples of 16 bytes, those between tokens at most 16 MiB, and all
+ * tensors' addresses are multiples of 16 bytes. A call that takes 2^32 threads
+ * or more in one launch is refused. No counterpart
  * in the reference (its tensors are packed) here and in the rest of this section. */
 typedef struct afhip_strides {
   int64_t batch, token, head;
@@ -534,14 +536,25 @@ AFHIP_API int afhip_rotary_backward(const afhip_rotary_desc* desc, const void* q
 /* Attention over a window of keys and the first few ("sinks"). Queries are the
  * last of their sequence: query i has position p = key_length - query_length +
  * i, and sees key j where j < key_length, j <= p + right, and j >= p - left or
- * j < sinks. Query head h reads key head h / (query_heads / key_heads). */
+ * j < sinks. Query head h reads key head h / (query_heads / key_heads).
+ *
+ * f32 values enter the products as three bf16 that hold all their bits, and
+ * the six largest of the nine products count (what is left out is below
+ * 2^-21 of the whole); an infinity counts as NaN there, and values below
+ * 2^-110 lose bits. f16 ones enter as they are, the probabilities rounded to
+ * f16. Sums are f32.
+ *
+ * Keys that no query of a sequence sees may hold anything. An infinity or a
+ * NaN that some query sees, in a value or on the way back in the gradient of
+ * a row, may reach the other queries and keys of the same sequence and key
+ * head that share its products, as zero times it. */
 typedef struct afhip_window_desc {
   int32_t batch, queries, keys; /* keys: rows of k and v, a cache's capacity for instance */
   int32_t query_heads, key_heads;
   int32_t head_dim;    /* a multiple of 8, at most 128 */
   int32_t left, right; /* -1: no end on that side */
   int32_t sinks;
-  int32_t dtype;       /* AFHIP_F32 | AFHIP_F16; products and sums in f32 */
+  int32_t dtype;       /* AFHIP_F32 | AFHIP_F16 */
   float scale;         /* on q . k, positive */
   afhip_strides q, k, v, out;
 } afhip_window_desc;

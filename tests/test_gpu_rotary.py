@@ -397,3 +397,6 @@ def test_refusals(dev):
                 dict(frequencies=np.ones(3))):
         with pytest.raises(_lib.RangeError):
             rotary.HeadRotary(4, 2, 32, **{"dtype": "f16", **bad})
+    many = torch.zeros(1, 1, 1, 8, dtype=q.dtype, device=dev).expand(1 << 23, 1, 1, 8)
+    with pytest.raises(_lib.RangeError, match="too many for one launch"):
+        rotary.HeadRotary(1, 1, 8, dtype="f16")(many, many)

@@ -186,7 +186,36 @@ CASES = [
     (1, 40, 40, 2, 2, 64, 3, 0, 100, None, None),             # sinks past the last key
     (2, 31, 95, 4, 4, 128, 1000, 1000, 0, [0, 31], [95, 64]),  # windows past both ends
     (1, 130, 130, 66, 1, 32, 40, 0, 2, None, None),           # one key head for 66
+    (2, 350, 350, 6, 2, 64, None, 0, 0, [350, 200], [350, 200]),  # groups of 3, the rows of a key in chunks
+    (1, 400, 400, 3, 1, 128, 50, 5, 300, None, None),         # sinks over some tiles of keys
+    (1, 300, 420, 2, 1, 32, 40, None, 0, None, None),         # all that follow
+    (1, 300, 420, 2, 1, 128, None, 30, 0, [290], [410]),      # all that came before
 ]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("head_dim", [32, 64, 128])
+def test_first_call_in_a_capture(head_dim, dtype, dev):
+    # Nothing has run these kernels before, in this file's order: what they set up once does not disturb a capture.
+    import torch
+
+    from afhip import window
+
+    rng, dt = np.random.default_rng(21), torch_dtype(dtype)
+    op = window.WindowAttention(4, 2, head_dim, left=60, sinks=2, dtype=dtype)
+    q, k, v, dout = (normal(rng, dev, dt, 1, 150, h, head_dim) for h in (4, 2, 2, 4))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = op(q, k, v, return_lse=True)
+        grads = op.backward(q, k, v, out, lse, dout)
+    for _ in range(3):
+        for x in (q, k, v, dout):
+            x.copy_(normal(rng, dev, dt, *x.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, want_lse = op(q, k, v, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        assert all(torch.equal(x, y) for x, y in zip(grads, op.backward(q, k, v, want, want_lse, dout)))
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
@@ -218,6 +247,126 @@ def test_split_keys(shape, dtype, dev):
     compare(op, q, k, v, None, None if b == 1 else [tk - 7, 0], dtype, dev, None, 0, 0, backward=False, what=shape)
     # So short that most parts have no block.
     compare(op, q, k, v, None, [min(tk, 37)] * b, dtype, dev, None, 0, 0, backward=False, what=("short", shape))
+
+
+def sampled(op, q, k, v, ql, kl, dtype, dev, left, right, sinks, pairs, backward=True, what=""):
+    """A large call, and the way back, at some sequences' key heads against the formulas; the same bits again."""
+    import torch
+
+    qi, ki = ints(ql, dev), ints(kl, dev)
+    out, lse = op(q, k, v, query_lengths=qi, key_lengths=ki, return_lse=True)
+    assert torch.equal(out, op(q, k, v, query_lengths=qi, key_lengths=ki))
+    dout = grads = None
+    if backward:
+        dout = normal(np.random.default_rng(99), dev, q.dtype, *q.shape)
+        grads = op.backward(q, k, v, out, lse, dout, query_lengths=qi, key_lengths=ki)
+        twice = op.backward(q, k, v, out, lse, dout, query_lengths=qi, key_lengths=ki)
+        assert all(torch.equal(x, y) for x, y in zip(grads, twice))
+    group = q.shape[2] // k.shape[2]
+    for i, kv in pairs:
+        heads, one = slice(kv * group, (kv + 1) * group), slice(kv, kv + 1)
+        s = Sequence(f64(q[i, :, heads]), f64(k[i, :, one]), f64(v[i, :, one]), q.shape[1] if ql is None else ql[i],
+                     k.shape[1] if kl is None else kl[i], left, right, sinks, op.scale, dtype,
+                     dout=None if dout is None else f64(dout[i, :, heads]))
+        holds(out[i, :, heads], s.out, s.out_tol, (what, i, kv, "out"))
+        holds(lse[i, heads].T, s.lse, s.lse_tol, (what, i, kv, "lse"))
+        if backward:
+            for name, x, part in zip(("dq", "dk", "dv"), grads, (heads, one, one)):
+                holds(x[i, :, part], getattr(s, name), getattr(s, name + "_tol"), (what, i, kv, name))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("head_dim", [32, 64, 128])
+@pytest.mark.parametrize("batch, group", [(8, 1), (32, 1), (32, 2)])
+def test_many_tiles(batch, group, head_dim, dtype, dev):
+    # 128, 512 and 1,024 tiles of 128 rows: where there are many, a workgroup has fewer waves.
+    from afhip import window
+
+    print("window tiles", dtype, batch, group, head_dim, flush=True)
+    rng, dt = np.random.default_rng(18), torch_dtype(dtype)
+    mask = dict(left=None, right=0, sinks=0) if group == 1 else dict(left=50, right=7, sinks=3)
+    op = window.WindowAttention(8 * group, 8, head_dim, dtype=dtype, **mask)
+    q = normal(rng, dev, dt, batch, 200, 8 * group, head_dim)
+    k, v = (normal(rng, dev, dt, batch, 230, 8, head_dim) for _ in range(2))
+    ql, kl = [200 - 7 * i % 90 for i in range(batch)], [230 - 11 * i % 120 for i in range(batch)]
+    pairs = [(0, 0), (batch // 2, 5), (batch - 1, 7)]
+    sampled(op, q, k, v, ql, kl, dtype, dev, *mask.values(), pairs, what=(batch, group, head_dim))
+
+
+@pytest.mark.parametrize("dtype, head_dim, batch", [("f16", 32, 8), ("f16", 64, 8), ("f16", 128, 2), ("f32", 32, 32),
+                                                    ("f32", 64, 8), ("f32", 128, 8)])
+def test_split_keys_of_many_rows(dtype, head_dim, batch, dev):
+    from afhip import window
+
+    print("window split rows", dtype, head_dim, batch, flush=True)
+    rng, dt = np.random.default_rng(19), torch_dtype(dtype)
+    op = window.WindowAttention(8, 8, head_dim, left=1300, sinks=40, dtype=dtype)
+    q = normal(rng, dev, dt, batch, 100, 8, head_dim)
+    k, v = (normal(rng, dev, dt, batch, 1500, 8, head_dim) for _ in range(2))
+    ql, kl = [100, 0] + [100 - 3 * i for i in range(2, batch)], [1500, 700] + [1500 - 45 * i for i in range(2, batch)]
+    pairs = [(0, 0), (1, 3), (batch - 1, 7)]
+    sampled(op, q, k, v, ql, kl, dtype, dev, 1300, 0, 40, pairs, backward=False, what=(dtype, head_dim))
+
+
+def test_f32_keeps_its_range(dev):
+    # Values of 2^-100 and 2^100, queries and keys of 2^60 and 2^-60: three bf16 of each hold all their bits.
+    from afhip import window
+
+    rng = np.random.default_rng(20)
+    op = window.WindowAttention(2, 1, 64, left=70, dtype="f32")
+    for sizes in ((0, 0, -100), (0, 0, 100), (60, -60, 0), (-60, 60, -40)):
+        q, k, v = (normal(rng, dev, torch_dtype("f32"), 1, 150, h, 64, scale=2.0 ** n)
+                   for h, n in zip((2, 1, 1), sizes))
+        compare(op, q, k, v, None, None, "f32", dev, 70, 0, 0, what=sizes)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_a_nan_stays_in_its_sequence_and_head(dtype, dev):
+    import torch
+
+    from afhip import window
+
+    rng, dt = np.random.default_rng(22), torch_dtype(dtype)
+    for tq, tk in ((150, 200), (1, 4000)):
+        op = window.WindowAttention(4, 2, 64, dtype=dtype)
+        q, k, v = (normal(rng, dev, dt, 2, n, h, 64) for n, h in ((tq, 4), (tk, 2), (tk, 2)))
+        dout = normal(rng, dev, dt, 2, tq, 4, 64)
+        want, want_lse = op(q, k, v, return_lse=True)
+        grads = op.backward(q, k, v, want, want_lse, dout)
+        v[1, 5, 1], k[1, 7, 1] = math.nan, math.inf
+        out, lse = op(q, k, v, return_lse=True)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1, :, :2], want[1, :, :2])
+        assert torch.isnan(out[1, :, 2:]).all() if tq == 1 else torch.isnan(out[1, -1, 2:]).all()
+        for x, y, heads in zip(op.backward(q, k, v, out, lse, dout), grads, (2, 1, 1)):
+            assert torch.equal(x[0], y[0]) and torch.equal(x[1, :, :heads], y[1, :, :heads])
+
+
+def test_two_streams_at_once(dev):
+    import torch
+
+    from afhip import window
+
+    rng, dt = np.random.default_rng(23), torch.float16
+    op = window.WindowAttention(8, 2, 128, dtype="f16")
+    calls = [[normal(rng, dev, dt, 1, n, h, 128) for n, h in ((80, 8), (5000, 2), (5000, 2), (80, 8))]
+             for _ in range(2)]
+
+    def run(q, k, v, dout):
+        out, lse = op(q, k, v, return_lse=True)
+        return out, lse, *op.backward(q, k, v, out, lse, dout)
+
+    want = [run(*x) for x in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for n, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[n].append(run(*calls[n]))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for x in a:
+            assert all(torch.equal(s, t) for s, t in zip(x, b))
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
@@ -482,3 +631,6 @@ def test_refusals(dev):
     for heads in ((4, 3, 32), (4, 2, 33), (4, 2, 136), (4, 2, 0), (0, 1, 32)):
         with pytest.raises(_lib.RangeError):
             window.WindowAttention(*heads)
+    many = torch.zeros(1, 1, 1, 8, dtype=dt, device=dev).expand(1 << 24, 1, 1, 8)
+    with pytest.raises(_lib.RangeError, match="too many for one launch"):
+        window.WindowAttention(1, 1, 8, dtype="f16")(many, many, many)

@@ -102,6 +102,13 @@ def test_workspaces():
     assert size("afhip_window_workspace_size", window(batch=1, queries=1, keys=40000, left=100)) == 0
     # The way back keeps 16 bytes a row.
     assert size("afhip_window_backward_workspace_size", window()) >= 2 * 5 * 4 * 16
+    # Only tiles of keys that every row sees, here those of the sinks, are cut into chunks of rows: 16 bytes a row, and
+    # the sums of two tiles of 128 keys in at most 64 chunks.
+    long = dict(batch=1, queries=131072, keys=131072, query_heads=32, key_heads=8, head_dim=128, left=1023)
+    rows = 131072 * 32 * 16
+    assert size("afhip_window_backward_workspace_size", window(**long, sinks=0)) == rows
+    sinks = size("afhip_window_backward_workspace_size", window(**long, sinks=200))
+    assert rows < sinks <= rows + 8 * 2 * 64 * 2 * 128 * 128 * 4
     assert size("afhip_rotary_backward_workspace_size", rotary(norm=0)) == 0
     assert size("afhip_rotary_backward_workspace_size", rotary(norm=2)) > 0
 
