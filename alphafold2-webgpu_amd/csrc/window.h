@@ -272,6 +272,7 @@ __device__ __forceinline__ void hide(int first, int lane, int low, int high, int
     for (int v = 0; v < 16; v++) {
       const bool hidden = 8 * (v >> 2) + (v & 3) >= to;
       ((x[v] = hidden ? fill : x[v]), ...);
+      if (v == 7) __builtin_amdgcn_sched_barrier(0);  // sixteen masks would fill the scalar registers
     }
   }
   if (starts) {
@@ -282,6 +283,7 @@ __device__ __forceinline__ void hide(int first, int lane, int low, int high, int
       const int at = 8 * (v >> 2) + (v & 3);
       const bool hidden = min(from - at, at - few + 1) > 0;
       ((x[v] = hidden ? fill : x[v]), ...);
+      if (v == 7) __builtin_amdgcn_sched_barrier(0);
     }
   }
 }

@@ -12,6 +12,11 @@
 // In f16, P goes into its product times 2^13 (the smallest of a row of 10^6 equal ones is then a normal number), and
 // ds, whose size nothing bounds, times a power of two that each held row (or key) lowers when a value would pass 2^15:
 // the accumulators are rescaled with it.
+//
+// Rounded to f16 the row's out makes D, and with it a whole row of ds, wrong by as much as ds' own rounding does where
+// a row sees few keys: dq 1.5 to 1.75 times as far from the truth as its own rounding to f16 alone, for 20 to 1,000
+// tokens. So dq takes ds as two f16, the rounded one and the rest (an MFMA more for four; 1.1 to 1.4 then), and sums
+// ds in f32: the sum is D's error, P having the sum 1, and dk and dv's kernel gets the D that is right.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -24,38 +29,23 @@ namespace {
 
 template <typename T> constexpr int kBlock = sizeof(T) == 2 ? 64 : 32;  // keys or rows of a streamed block
 
-// A held row's power of two on ds (f16), and the accumulators it is on.
-template <typename T, int BLOCKS> struct Scaled {
-  floatx16 acc[BLOCKS];
-  float scale;
-
-  __device__ __forceinline__ void init() {
+// The power of two (f16) that brings a held row's, or key's, largest ds of a block to [2^7, 2^8).
+__device__ __forceinline__ float fitting(float top) {
+  const float both = fmaxf(top, __shfl_xor(top, 32));
+  return ldexpf(1.0f, min(126, 8 - __builtin_amdgcn_frexp_expf(both)));
+}
+__device__ __forceinline__ float largest(const float* ds) {
+  float top = fabsf(ds[0]);
 #pragma unroll
-    for (int c = 0; c < BLOCKS; c++) acc[c] = floatx16{};
-    scale = sizeof(T) == 2 ? 0x1p126f : 1.0f;
-  }
-  // Brings ds into f16's range.
-  __device__ __forceinline__ void fit(float* ds) {
-    if constexpr (sizeof(T) == 2) {
-      float top = fabsf(ds[0]);
+  for (int v = 1; v < 16; v++) top = fmaxf(top, fabsf(ds[v]));
+  return top;
+}
+template <int BLOCKS> __device__ __forceinline__ void times(floatx16* acc, float f) {
 #pragma unroll
-      for (int v = 1; v < 16; v++) top = fmaxf(top, fabsf(ds[v]));
-      if (__builtin_amdgcn_ballot_w64(top * scale > 0x1p15f)) {
-        const float both = fmaxf(top, __shfl_xor(top, 32));
-        // To [2^7, 2^8).
-        const float to = ldexpf(1.0f, min(126, 8 - __builtin_amdgcn_frexp_expf(both)));
-        const float next = both > 0.0f ? fminf(to, scale) : scale, f = next / scale;
+  for (int c = 0; c < BLOCKS; c++)
 #pragma unroll
-        for (int c = 0; c < BLOCKS; c++)
-#pragma unroll
-          for (int v = 0; v < 16; v++) acc[c][v] *= f;
-        scale = next;
-      }
-#pragma unroll
-      for (int v = 0; v < 16; v++) ds[v] *= scale;
-    }
-  }
-};
+    for (int v = 0; v < 16; v++) acc[c][v] *= f;
+}
 
 // dq, and each row's lse and D for the other kernel. ROWS waves of 32 rows each, and PARTS times as many where there
 // are few rows: each part takes its WK keys of every block, and the parts' sums meet in LDS.
@@ -64,7 +54,7 @@ template <typename T, int DP, int ROWS, int PARTS, int WK> struct RowTile {
   static constexpr int kLds = 4 * PARTS * WK * DP * (int)sizeof(T);
   // Workgroups a CU, for its LDS; the widest f32 takes more than 256 registers.
   static constexpr int kGroups = kLds > 81920 || DP * sizeof(T) > 256 ? 1 : 2;
-  static_assert(PARTS == 1 || (PARTS - 1) * ROWS * DP * 128 <= kLds, "the other parts' sums fit");
+  static_assert(PARTS == 1 || (PARTS - 1) * ROWS * (DP * 128 + 256) <= kLds, "the other parts' sums fit");
 };
 
 template <typename T, int DP, int ROWS, int PARTS, int WK>
@@ -73,6 +63,7 @@ __launch_bounds__((RowTile<T, DP, ROWS, PARTS, WK>::kThreads), (RowTile<T, DP, R
 void window_dq_kernel(WindowArgs a) {
   constexpr int BK = WK * PARTS, STEPS = DP / 16, BLOCKS = DP / 32;
   constexpr int HELD = RowTile<T, DP, ROWS, PARTS, WK>::kRows;
+  constexpr bool F16 = sizeof(T) == 2;
   typedef TileLoad<T, DP, BK, ROWS * PARTS> Load;
   typedef typename Eight<T>::type Frag;
   typedef Tile<T, DP> Tl;
@@ -119,7 +110,9 @@ void window_dq_kernel(WindowArgs a) {
   if (total > 0) issue(0);
 
   Frag q[STEPS], g[STEPS];
-  float delta = 0.0f, lse = INFINITY;
+  float delta = 0.0f;
+  float* left_delta;
+  float lse = INFINITY;
   {
     const int64_t src = live ? i : 0;
     const char* qp = a.q + b * a.sq.batch + src * a.sq.token + h * a.sq.head;
@@ -141,13 +134,22 @@ void window_dq_kernel(WindowArgs a) {
       lse = a.lse[((int64_t)b * a.query_heads + h) * a.queries + i] * kWindowLog2e;
       if (lse == -INFINITY) lse = INFINITY;  // nothing seen: probabilities of 0
     }
+    left_delta = &a.rows[(int64_t)pair * rows + row].y;
     if (row < rows && !hi && part == 0) {
       a.rows[(int64_t)pair * rows + row] = float2{lse, delta};
       a.limits[(int64_t)pair * rows + row] = live ? int2{high, low} : int2{0, 0};
     }
   }
-  Scaled<T, BLOCKS> acc;
-  acc.init();
+  // As a factor that the compiler does not see, it makes a difference and its rounding to f16 one instruction.
+  float one = 1.0f;
+  asm("" : "+s"(one));
+  float rest = 0.0f;  // f16: the sum of the row's ds, which is what out's rounding put D off by
+  // ds comes from the exponential with its power of two. The first holds the product of any f16 dout and v.
+  int shift = F16 ? 60 : 0;
+  float from = (float)shift - lse;
+  floatx16 acc[BLOCKS];
+#pragma unroll
+  for (int c = 0; c < BLOCKS; c++) acc[c] = floatx16{};
   // As in window_rows_kernel.
   const auto phases =
       range.phases(0, total, BK, s.low(a, wfirst), s.high(a, wlast), wr0 < s.queries * a.group);
@@ -161,7 +163,7 @@ void window_dq_kernel(WindowArgs a) {
       const bool ends = k0 + WK > all_high, starts = k0 < all_low && k0 + WK > range.sinks;
       const unsigned char* kt = smem + (t & 1) * 2 * Load::kBytes + at * Tl::kRow;
       const unsigned char* vt = kt + Load::kBytes;
-#pragma unroll
+#pragma unroll 1
       for (int sub = 0; sub < WK; sub += 32) {
         floatx16 x = floatx16{}, y = floatx16{};
 #pragma unroll
@@ -172,43 +174,70 @@ void window_dq_kernel(WindowArgs a) {
         float ds[16];
 #pragma unroll
         for (int v = 0; v < 16; v++)
-          ds[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, -lse)) * (y[v] - delta);
+          ds[v] = __builtin_amdgcn_exp2f(fmaf(x[v], a.scale_log2, from)) * (y[v] - delta);
         if (ends | starts) hide(k0 + sub, lane, low, high, range.sinks, ends, starts, 0.0f, ds);
-        acc.fit(ds);
+        if constexpr (F16) {
+          const float top = largest(ds);
+          if (__builtin_amdgcn_ballot_w64(top > 0x1p15f)) {
+            const float f = fminf(fitting(top), 1.0f);
+            times<BLOCKS>(acc, f);
+            rest *= f;
+#pragma unroll
+            for (int v = 0; v < 16; v++) ds[v] *= f;
+            const int by = __builtin_amdgcn_frexp_expf(f) - 1;
+            shift += by;
+            from += (float)by;
+          }
+          rest += (((ds[0] + ds[1]) + (ds[2] + ds[3])) + ((ds[4] + ds[5]) + (ds[6] + ds[7]))) +
+                  (((ds[8] + ds[9]) + (ds[10] + ds[11])) + ((ds[12] + ds[13]) + (ds[14] + ds[15])));
+        }
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-          const Frag f = pack8(ds + 8 * n, (Frag*)nullptr);
+          Frag f = pack8(ds + 8 * n, (Frag*)nullptr), g;
+          if constexpr (F16) {
+            asm("" : "+v"(f));  // else each half is rounded once more
 #pragma unroll
-          for (int c = 0; c < BLOCKS; c++) acc.acc[c] = mma(Tl::tr(kt, sub + 16 * n, c, lane), f, acc.acc[c]);
+            for (int j = 0; j < 8; j++) g[j] = (half_t)fmaf(ds[8 * n + j], one, -(float)f[j]);
+          }
+#pragma unroll
+          for (int c = 0; c < BLOCKS; c++) {
+            const Frag k = Tl::tr(kt, sub + 16 * n, c, lane);
+            if constexpr (F16) acc[c] = mma(k, g, acc[c]);
+            acc[c] = mma(k, f, acc[c]);
+          }
         }
       }
     }
     for (; t < idle; t++) arrive(t);
   }
-  const float f = a.scale / acc.scale;
-#pragma unroll
-  for (int c = 0; c < BLOCKS; c++)
-#pragma unroll
-    for (int v = 0; v < 16; v++) acc.acc[c][v] *= f;
+  times<BLOCKS>(acc, ldexpf(a.scale, -shift));
+  if (F16) rest = ldexpf(rest, -shift);
   if constexpr (PARTS > 1) {
+    constexpr int SUMS = (PARTS - 1) * ROWS * BLOCKS * 1024;  // then the rests
     float* shared = reinterpret_cast<float*>(smem) + rg * BLOCKS * 1024 + lane;
+    float* rests = reinterpret_cast<float*>(smem) + SUMS + rg * 64 + lane;
     block_barrier();  // the last block is read
     if (part > 0) {
+      rests[(part - 1) * ROWS * 64] = rest;
 #pragma unroll
       for (int c = 0; c < BLOCKS; c++)
 #pragma unroll
-        for (int v = 0; v < 16; v++) shared[((part - 1) * ROWS * BLOCKS * 16 + 16 * c + v) * 64] = acc.acc[c][v];
+        for (int v = 0; v < 16; v++) shared[((part - 1) * ROWS * BLOCKS * 16 + 16 * c + v) * 64] = acc[c][v];
     }
     block_barrier();
     if (part > 0) return;
 #pragma unroll 1
-    for (int p = 0; p < PARTS - 1; p++)
+    for (int p = 0; p < PARTS - 1; p++) {
+      rest += rests[p * ROWS * 64];
 #pragma unroll
       for (int c = 0; c < BLOCKS; c++)
 #pragma unroll
-        for (int v = 0; v < 16; v++) acc.acc[c][v] += shared[(p * ROWS * BLOCKS * 16 + 16 * c + v) * 64];
+        for (int v = 0; v < 16; v++) acc[c][v] += shared[(p * ROWS * BLOCKS * 16 + 16 * c + v) * 64];
+    }
   }
+  if (F16) rest += __shfl_xor(rest, 32);
   if (row >= rows) return;
+  if (F16 && !hi) *left_delta = delta + rest;
   T* to = reinterpret_cast<T*>(a.dq) + (((int64_t)b * a.queries + i) * a.query_heads + h) * a.head_dim;
 #pragma unroll
   for (int c = 0; c < BLOCKS; c++)
@@ -216,7 +245,7 @@ void window_dq_kernel(WindowArgs a) {
     for (int g = 0; g < 4; g++) {
       const int ch = 32 * c + 8 * g + 4 * hi;
       if (ch >= a.head_dim) continue;
-      const floatx16& x = acc.acc[c];
+      const floatx16& x = acc[c];
       put4(to + ch, live ? x[4 * g] : 0.0f, live ? x[4 * g + 1] : 0.0f, live ? x[4 * g + 2] : 0.0f,
            live ? x[4 * g + 3] : 0.0f);
     }
@@ -272,7 +301,8 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
   constexpr int BR = KT::kRows, STEPS = DP / 16, BLOCKS = DP / 32, WAVES = KT::kThreads / 64;
   constexpr int CHUNKS = Tl::kChunks, STEP = 64 / CHUNKS, COUNT = BR * CHUNKS / 64;
   constexpr int TILE = KT::kTileBytes;
-  constexpr float LIFT = sizeof(T) == 2 ? 13.0f : 0.0f;  // on P's exponent, and so on ds
+  constexpr bool F16 = sizeof(T) == 2;
+  constexpr float LIFT = F16 ? 13.0f : 0.0f;  // on P's exponent, and so on ds
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -291,11 +321,10 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
   const int begin = range.begin + chunk * a.chunk_rows, stop = min(range.stop, begin + a.chunk_rows);
 
   const unsigned char* vt = smem + 2 * KT::kBuffer;
-  Scaled<T, BLOCKS> dk;
-  floatx16 dv[BLOCKS];
-  dk.init();
+  floatx16 dk[BLOCKS], dv[BLOCKS];
+  float dk_scale = F16 ? 0x1p126f : 1.0f;
 #pragma unroll
-  for (int c = 0; c < BLOCKS; c++) dv[c] = floatx16{};
+  for (int c = 0; c < BLOCKS; c++) dk[c] = dv[c] = floatx16{};
 
   if (begin < stop) {
     int wfirst, wend;
@@ -458,21 +487,30 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
 #pragma unroll
           for (int v = 0; v < 16; v++) ds[v] = p[v] == 0.0f ? 0.0f : ds[v];
         }
-        dk.fit(ds);
+        if constexpr (F16) {
+          const float top = largest(ds);
+          if (__builtin_amdgcn_ballot_w64(top * dk_scale > 0x1p15f)) {
+            const float next = fminf(fitting(top), dk_scale);
+            times<BLOCKS>(dk, next / dk_scale);
+            dk_scale = next;
+          }
+#pragma unroll
+          for (int v = 0; v < 16; v++) ds[v] *= dk_scale;
+        }
 #pragma unroll
         for (int m = 0; m < 2; m++) {
           const Frag pf = pack8(p + 8 * m, (Frag*)nullptr), df = pack8(ds + 8 * m, (Frag*)nullptr);
 #pragma unroll
           for (int c = 0; c < BLOCKS; c++) {
             dv[c] = mma(Tl::tr(gt, sub + 16 * m, c, lane), pf, dv[c]);
-            dk.acc[c] = mma(Tl::tr(qt, sub + 16 * m, c, lane), df, dk.acc[c]);
+            dk[c] = mma(Tl::tr(qt, sub + 16 * m, c, lane), df, dk[c]);
           }
         }
       }
     }
   }
   // The row groups' sums, in their own magnitude, meet in LDS, one gradient at a time, and leave as whole rows.
-  const float fv = sizeof(T) == 2 ? 0x1p-13f : 1.0f, fk = a.scale * fv / dk.scale;
+  const float fv = F16 ? 0x1p-13f : 1.0f, fk = a.scale * fv / dk_scale;
   constexpr int PITCH = DP + 4;
   static_assert(KT::kKeys * PITCH * 4 <= KT::kLds, "a gradient of the tile fits");
   float* shared = reinterpret_cast<float*>(smem);
@@ -509,7 +547,7 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
       }
     }
   };
-  leave(dk.acc, fk, 0);
+  leave(dk, fk, 0);
   leave(dv, fv, 1);
 }
 
