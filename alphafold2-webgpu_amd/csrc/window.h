@@ -31,9 +31,9 @@ struct WindowArgs {
   // [batch][key head][row]: the row's lse in base 2 and the sum of out * dout; the keys it sees, below and from.
   float2* rows;
   int2* limits;
-  // dk and dv: the most chunks of rows that a tile of keys has, the rows of one; tiles that all rows may see, and the
-  // chunks of the others.
-  int chunks, chunk_rows, long_tiles, short_chunks;
+  // dk and dv: tiles of keys that every row may see, and the most chunks of rows that one of them and of the others
+  // has; the rows of a chunk, and of one where sinks are.
+  int long_tiles, chunks, short_chunks, chunk_rows, sink_rows;
   int parts;  // chunks of a key head that leave partial sums
 };
 

@@ -273,13 +273,14 @@ template <typename T, int DP> struct KeyTile {
 
 // Rows that see any key of a tile, and its chunks of them.
 struct TileRows {
-  int begin, stop, chunks;
+  int begin, stop, chunk_rows, chunks;
   __device__ __forceinline__ TileRows(const WindowArgs& a, const Sequence& s, int from, int to) {
     int first, end;
     queries(a, s, from, to, first, end);
     begin = first * a.group;
     stop = max(begin, end * a.group);
-    chunks = (stop - begin + a.chunk_rows - 1) / a.chunk_rows;
+    chunk_rows = from < a.sinks ? a.sink_rows : a.chunk_rows;
+    chunks = (stop - begin + chunk_rows - 1) / chunk_rows;
   }
   // Queries [first, end) that see any of keys [from, to).
   static __device__ __forceinline__ void queries(const WindowArgs& a, const Sequence& s, int from, int to, int& first,
@@ -318,7 +319,7 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
   const bool live = key < s.keys;
   const TileRows range(a, s, j0, j0 + KT::kKeys);
   if (chunk > 0 && chunk >= range.chunks) return;
-  const int begin = range.begin + chunk * a.chunk_rows, stop = min(range.stop, begin + a.chunk_rows);
+  const int begin = range.begin + chunk * range.chunk_rows, stop = min(range.stop, begin + range.chunk_rows);
 
   const unsigned char* vt = smem + 2 * KT::kBuffer;
   floatx16 dk[BLOCKS], dv[BLOCKS];
@@ -577,7 +578,7 @@ __global__ __launch_bounds__(256) void window_dkv_join_kernel(WindowArgs a, int 
 
 // The key tiles, and the rows of a chunk.
 struct KeyPlan {
-  int tile_keys, tiles, chunk_rows;
+  int tile_keys, tiles, chunk_rows, sink_rows;
   int long_tiles, chunks, short_chunks;  // tiles that every row may see, the chunks of one, those of the others
   int64_t groups(int64_t heads) const {
     return heads * ((int64_t)long_tiles * chunks + (int64_t)(tiles - long_tiles) * short_chunks);
@@ -591,23 +592,40 @@ struct KeyPlan {
 
 KeyPlan key_plan(const afhip_window_desc& d) {
   KeyPlan p{};
-  const bool wide = d.head_dim > 32 && d.dtype == AFHIP_F32;
+  const bool f32 = d.dtype == AFHIP_F32, wide = d.head_dim > 32 && f32;
   p.tile_keys = wide ? KeyTile<float, 128>::kKeys : KeyTile<half_t, 128>::kKeys;
   p.tiles = (int)ceil_div(d.keys, p.tile_keys);
-  const int64_t group = d.query_heads / d.key_heads, all = d.queries * group;
-  // Rows that see a tile, without sinks.
-  const int64_t span = d.left < 0 || d.right < 0
-                           ? all : std::min<int64_t>(all, ((int64_t)d.left + d.right + p.tile_keys) * group);
-  const int64_t most = d.left < 0 || d.sinks > 0 ? all : span, groups = (int64_t)d.batch * d.key_heads * p.tiles;
+  const int64_t group = d.query_heads / d.key_heads, all = d.queries * group, heads = (int64_t)d.batch * d.key_heads;
+  // Rows that see a tile, without sinks; without a window on both sides all, or half of them on average.
+  const bool window = d.left >= 0 && d.right >= 0, half = !window && (d.left >= 0 || d.right >= 0);
+  const int64_t span = window ? std::min<int64_t>(all, ((int64_t)d.left + d.right + p.tile_keys) * group) : all;
+  const bool sinks = d.left >= 0 && d.sinks > 0;
   p.long_tiles = d.left < 0 ? p.tiles : (int)std::min<int64_t>(p.tiles, ceil_div(d.sinks, p.tile_keys));
-  // Chunks that make about 400 workgroups: with one a CU, fewer leave CUs idle at the end, more cost each a start and
-  // sums to join. 4,096 tokens, 16 heads over 4, window 1,024, dk and dv with the join in us on MI355X: 256 workgroups
-  // 154, 300 150, 350 139, 400 134, 512 159, 600 146, 800 156, 1,000 191.
-  int64_t rows = std::max<int64_t>(ceil_div(span * groups, 400), 128);
-  rows = std::max(rows, ceil_div(most, 64));
-  p.chunk_rows = (int)round_up(rows, 64);
-  p.chunks = (int)ceil_div(most, p.chunk_rows);
-  p.short_chunks = (int)ceil_div(span, p.chunk_rows);
+  // The chunks that take the shortest by what they cost on MI355X in us, a CU having one workgroup at a time: a block
+  // of 64 rows (f16 2.8 over 128 channels, f32 9), a workgroup's start and end, the join and its sums at 4 TB/s. dk, dv
+  // and the join for 4,096 tokens, 16 heads over 4 of 128 channels, f16, window 1,024: 3 chunks of each tile 137, 2 102;
+  // with 4 sinks, whose tile every row sees, 1 to 5 chunks 191, 166, 146, 169, 156.
+  const int width = d.head_dim <= 32 ? 32 : d.head_dim <= 64 ? 64 : 128;
+  const double block = f32 ? std::max(3.5, 0.07 * width) : 0.022 * width, ends = f32 && width == 128 ? 25 : 8;
+  double best = INFINITY;
+  for (int64_t chunks = 1; chunks <= 64; chunks++) {
+    const int64_t rows = round_up(ceil_div(span, chunks), 64), each = ceil_div(span, rows);
+    if (chunks > 1 && rows < 128) break;
+    const int64_t sink_rows = std::max(rows, round_up(ceil_div(all, 64), 64));
+    const int64_t most = sinks ? ceil_div(all, sink_rows) : each;
+    const double one = ends + block * rows / 64;
+    const double groups = (double)heads * (p.long_tiles * most + (p.tiles - p.long_tiles) * each);
+    // Tiles of many lengths: what a CU has on average, and half a chunk for the end.
+    const double work = (groups + heads * p.tiles) / 2 * ends + (double)heads * p.tiles * block * span / 128;
+    double time = half ? std::max(one, work / 256 + one / 2) : std::ceil(groups / 256) * one;
+    if (each > 1 || most > 1) time += 4 + groups * 4 * p.tile_keys * d.head_dim * 4 / 4e6;
+    if (time >= best) continue;
+    best = time;
+    p.chunk_rows = (int)rows;
+    p.sink_rows = (int)sink_rows;
+    p.short_chunks = (int)each;
+    p.chunks = (int)std::max(each, most);
+  }
   return p;
 }
 
@@ -647,6 +665,7 @@ template <typename T, int DP> int launch_backward(WindowArgs& a, const KeyPlan& 
   a.tiles = p.tiles;
   a.chunks = p.chunks;
   a.chunk_rows = p.chunk_rows;
+  a.sink_rows = p.sink_rows;
   a.long_tiles = p.long_tiles;
   a.short_chunks = p.short_chunks;
   a.parts = (int)p.parts();
