@@ -269,8 +269,10 @@ __global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) >
 // every second CU, 18.8 us, 3.6 TB/s.
 template <typename T, int DP> struct Step {
   static constexpr int kBytes = 2 * 32 * DP * (int)sizeof(T);  // K and V of a block
-  static constexpr int kWaves = kBytes >= 32768 ? 2 : 4;
-  static constexpr int kStages = kBytes >= 16384 ? 2 : 4;
+  static constexpr int kWaves = 4;
+  // Four waves with one buffer each where two fill the LDS with two: 16 sequences of 4,000 keys, 8 heads of 128
+  // channels, f32, 131 us and 156; 2 of 195, 11 and 19.
+  static constexpr int kStages = kBytes >= 32768 ? 1 : kBytes >= 16384 ? 2 : 4;
   static constexpr int kLds = kWaves * kStages * kBytes;
   static_assert(kLds >= kWaves * 32 * (DP + 2) * 4, "the waves' sums fit");
 };
@@ -428,8 +430,8 @@ Plan plan(const afhip_window_desc& d) {
   const int64_t group = d.query_heads / d.key_heads, rows = d.queries * group, heads = (int64_t)d.batch * d.key_heads;
   Plan p{};
   // Tiles of 32 rows also where those of 128 are few. Whole calls on MI355X, tiles of 128 / 32, us: f32 over 32
-  // channels 128 tiles 15.9 / 10.1, 256 tiles 17.8 / 32; over 64 40 tiles 28 / 20, 64 tiles 35 / 37; over 128 20 tiles
-  // 39 / 36; f16 over 64 channels 2 tiles 10.5 / 8.9, 128 tiles 12.7 / 16.5; over 128 20 tiles 12.2 / 13.6.
+  // channels 128 tiles 15.9 / 10.1, 256 tiles 17.8 / 32; over 64 40 tiles 28 / 20, 64 tiles 35 / 37; over 128 40 tiles
+  // 33 / 34, 112 tiles 33 / 43; f16 over 64 channels 2 tiles 10.5 / 8.9, 128 tiles 12.7 / 16.5; over 128 20 tiles 12.2 / 13.6.
   const int64_t few = f32 ? (d.head_dim <= 32 ? 256 : 64) : d.head_dim <= 64 ? 64 : 0;
   p.step = rows <= 32 || heads * ceil_div(rows, kTileRows) < few;
   p.tiles = (int)ceil_div(rows, p.step ? 32 : kTileRows);
@@ -444,10 +446,10 @@ Plan plan(const afhip_window_desc& d) {
     span = std::min(span, (int64_t)d.left + right + queries + std::min<int64_t>(d.sinks, d.keys));
   }
   // Into how many parts the keys are split: the shortest of some, by what they take on MI355X in us. A block of 32 keys
-  // takes a workgroup 0.4 (f16, 128 channels; f32 2.6), a workgroup's start and end 4, a CU having one of them at a
+  // takes a workgroup 0.4 (f16, 128 channels; f32 2.6, of four waves with keys of their own 1.2), a workgroup's start and end 4, a CU having one of them at a
   // time; the keys' bytes come at 5.3 TB/s where all CUs ask for them, at 4 where half do; the join takes 4.5, and its
   // sums go out and in at 3.5 TB/s.
-  const double block = std::max((f32 ? 2.6 : 0.4) * d.head_dim / 128, 0.15);
+  const double block = std::max((!f32 ? 0.4 : p.step ? 1.2 : 2.6) * d.head_dim / 128, 0.15);
   const double bytes = 2.0 * heads * span * d.head_dim * dtype_size(d.dtype);
   double best = INFINITY;
   for (int64_t splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {

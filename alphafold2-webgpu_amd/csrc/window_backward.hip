@@ -53,7 +53,8 @@ template <int BLOCKS> __device__ __forceinline__ void times(floatx16* acc, float
 // TFLOP/s over its four products.
 template <typename T, int DP, int ROWS, int PARTS, int WK> struct RowTile {
   static constexpr int kRows = 32 * ROWS, kThreads = 64 * ROWS * PARTS;
-  static constexpr int kLds = 4 * PARTS * WK * DP * (int)sizeof(T);
+  static constexpr int kBlock = 2 * PARTS * WK * DP * (int)sizeof(T);  // K and V
+  static constexpr int kStages = kBlock > 81920 ? 1 : 2, kLds = kStages * kBlock;
   // Workgroups a CU, for its LDS; the widest f32 takes more than 256 registers.
   static constexpr int kGroups = kLds > 81920 || DP * sizeof(T) > 256 ? 1 : 2;
   static_assert(PARTS == 1 || (PARTS - 1) * ROWS * (DP * 128 + 256) <= kLds, "the other parts' sums fit");
@@ -64,7 +65,7 @@ __global__
 __launch_bounds__((RowTile<T, DP, ROWS, PARTS, WK>::kThreads), (RowTile<T, DP, ROWS, PARTS, WK>::kGroups))
 void window_dq_kernel(WindowArgs a) {
   constexpr int BK = WK * PARTS, STEPS = DP / 16, BLOCKS = DP / 32;
-  constexpr int HELD = RowTile<T, DP, ROWS, PARTS, WK>::kRows;
+  constexpr int HELD = RowTile<T, DP, ROWS, PARTS, WK>::kRows, STAGES = RowTile<T, DP, ROWS, PARTS, WK>::kStages;
   constexpr bool F16 = sizeof(T) == 2;
   typedef TileLoad<T, DP, BK, ROWS * PARTS> Load;
   typedef typename Eight<T>::type Frag;
@@ -98,16 +99,20 @@ void window_dq_kernel(WindowArgs a) {
   vload.init(wave, lane, a.head_dim, a.sv.token);
   auto issue = [&](int t) {
     const int k0 = range.block(t) * BK;
-    const uint32_t buffer = lds + (uint32_t)(t & 1) * 2 * Load::kBytes;
+    const uint32_t buffer = lds + (uint32_t)(t % STAGES) * 2 * Load::kBytes;
     const bool whole = range.whole(k0, BK);
     auto keep = [&](int key) { return range.keeps(key); };
     kload.issue(kb, a.sk.token, k0, buffer, wave, whole, keep);
     vload.issue(vb, a.sv.token, k0, buffer + Load::kBytes, wave, whole, keep);
   };
   auto arrive = [&](int t) {
+    if (STAGES == 1 && t > 0) {
+      block_barrier();  // block t - 1 is read
+      issue(t);
+    }
     wait_vmcnt<0>();
     block_barrier();
-    if (t + 1 < total) issue(t + 1);
+    if (STAGES == 2 && t + 1 < total) issue(t + 1);
   };
   if (total > 0) issue(0);
 
@@ -163,7 +168,7 @@ void window_dq_kernel(WindowArgs a) {
       arrive(t);
       const int at = WK * part, k0 = range.block(t) * BK + at;
       const bool ends = k0 + WK > all_high, starts = k0 < all_low && k0 + WK > range.sinks;
-      const unsigned char* kt = smem + (t & 1) * 2 * Load::kBytes + at * Tl::kRow;
+      const unsigned char* kt = smem + (t % STAGES) * 2 * Load::kBytes + at * Tl::kRow;
       const unsigned char* vt = kt + Load::kBytes;
 #pragma unroll 1
       for (int sub = 0; sub < WK; sub += 32) {
@@ -650,7 +655,7 @@ int launch_dq(WindowArgs& a, int64_t heads, int64_t rows, hipStream_t st) {
 // would leave most CUs with nothing.
 template <typename T, int DP> int launch_dq_any(WindowArgs& a, int64_t heads, int64_t rows, hipStream_t st) {
   constexpr int WK = kBlock<T>, EIGHT = DP * sizeof(T) > 256 ? 1 : 2;
-  constexpr int FEW = DP * sizeof(T) > 256 ? 2 : DP * sizeof(T) > 64 ? 4 : 8;
+  constexpr int FEW = DP * sizeof(T) > 64 ? 4 : 8;
   const int64_t groups = heads * ceil_div(rows, 128);
   if (groups < 128) return launch_dq<T, DP, 1, FEW, 32>(a, heads, rows, st);
   if (groups < 512) return launch_dq<T, DP, 4, EIGHT, WK>(a, heads, rows, st);
