@@ -16,8 +16,8 @@ struct WindowArgs {
   char* out;
   float* lse;
   const int32_t *query_lengths, *key_lengths;
-  // Split keys: [row][split] of head_dim sums, the reference point, the total. The way back: dk and dv of each chunk
-  // of the tiles that may have several.
+  // Split keys: [row][split] of head_dim sums, then of the reference point and the total. The way back: dk and dv of
+  // each chunk of the tiles that may have several.
   float* partial;
   HeadStrides sq, sk, sv, so;
   int batch, queries, keys, query_heads, key_heads, group, head_dim;

@@ -121,6 +121,13 @@ __device__ __forceinline__ int64_t lse_index(const WindowArgs& a, int b, int h, 
   return ((int64_t)b * a.query_heads + h) * a.queries + i;
 }
 
+constexpr int kJoinRows = 8;  // of a workgroup of window_join_kernel, which takes up to 64 splits
+
+// The reference points and totals of split keys, behind their sums.
+__device__ __forceinline__ float2* part_totals(const WindowArgs& a) {
+  return reinterpret_cast<float2*>(a.partial + (int64_t)a.batch * a.queries * a.query_heads * a.splits * a.head_dim);
+}
+
 // Four waves of 32 rows, or with PARTS = 2 eight, of which the second four take the second half of every block: where
 // there are few tiles, twice the waves for the same reads of K and V, and their sums meet in LDS.
 // MFMA bounds it, and the softmax's vector instructions, which a SIMD's two waves issue beside each other's MFMAs:
@@ -230,17 +237,17 @@ __global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) >
   const int i = row / a.group, h = kv * a.group + row % a.group;
   if constexpr (SPLIT) {
     const int64_t n = ((int64_t)pair * rows + row) * a.splits + split;
-    float* to = a.partial + n * (a.head_dim + 2);
+    float* to = a.partial + n * a.head_dim;
 #pragma unroll
     for (int c = 0; c < DP / 32; c++)
 #pragma unroll
       for (int g = 0; g < 4; g++) {
         const int ch = 32 * c + 8 * g + 4 * hi;
         if (ch >= a.head_dim) continue;
-#pragma unroll
-        for (int j = 0; j < 4; j++) to[ch + j] = st.o[c][4 * g + j];
+        const floatx16& o = st.o[c];
+        put4(to + ch, o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
       }
-    if (!hi) to[a.head_dim] = st.m, to[a.head_dim + 1] = l;
+    if (!hi) part_totals(a)[n] = float2{st.m, l};
   } else {
     const bool live = i < s.queries && l != 0.0f;
     const float inv = 1.0f / l;
@@ -361,9 +368,9 @@ __global__ __launch_bounds__((kStepThreads<T, DP>)) void window_step_kernel(Wind
     }
     const int i = (r0 + r) / a.group, h = kv * a.group + (r0 + r) % a.group;
     if (a.splits > 1) {
-      float* to = a.partial + (((int64_t)pair * all + r0 + r) * a.splits + split) * (a.head_dim + 2);
-      to[ch] = o;
-      if (ch == 0) to[a.head_dim] = m, to[a.head_dim + 1] = sum;
+      const int64_t to = ((int64_t)pair * all + r0 + r) * a.splits + split;
+      a.partial[to * a.head_dim + ch] = o;
+      if (ch == 0) part_totals(a)[to] = float2{m, sum};
     } else {
       const bool live = i < s.queries;
       T* to = reinterpret_cast<T*>(a.out + b * a.so.batch + i * a.so.token + h * a.so.head);
@@ -373,46 +380,56 @@ __global__ __launch_bounds__((kStepThreads<T, DP>)) void window_step_kernel(Wind
   }
 }
 
-// Joins the splits of a row, one wave a row and two channels a lane: 4 us, a launch's least, for single tokens; 6.4 for
-// 8,192 rows of 4 parts, 17 MB.
+// Joins the splits of a row, half a wave a row and four channels a lane: 4 us, a launch's least, for single tokens;
+// 4.8 for 8,192 rows of 4 parts, 17 MB.
 template <typename T> __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (int64_t)a.queries * a.group;
+  const int lane = threadIdx.x & 31;
+  const int64_t n = (int64_t)blockIdx.x * kJoinRows + (threadIdx.x >> 5), rows = (int64_t)a.queries * a.group;
   if (n >= (int64_t)a.batch * a.key_heads * rows) return;
   const int pair = (int)(n / rows), row = (int)(n % rows);
   const int b = pair / a.key_heads, kv = pair % a.key_heads, i = row / a.group, h = kv * a.group + row % a.group;
   const Sequence s(a, b);
-  const float* from = a.partial + n * a.splits * (a.head_dim + 2);
-  const float* at = from + (int64_t)min(lane, a.splits - 1) * (a.head_dim + 2) + a.head_dim;
-  const float mine = lane < a.splits ? at[0] : -INFINITY;
-  float m = mine;
+  // Two splits a lane; past the last one a total of 0.
+  const float2* totals = part_totals(a) + n * a.splits;
+  float2 mine[2];
 #pragma unroll
-  for (int step = 1; step < 64; step *= 2) m = fmaxf(m, __shfl_xor(m, step));
-  const float f = lane >= a.splits ? 0.0f : mine == m ? 1.0f : __builtin_amdgcn_exp2f(mine - m);
-  float total = lane < a.splits ? f * at[1] : 0.0f;
+  for (int j = 0; j < 2; j++) {
+    mine[j] = totals[min(lane + 32 * j, a.splits - 1)];
+    if (lane + 32 * j >= a.splits) mine[j] = float2{-INFINITY, 0.0f};
+  }
+  float m = fmaxf(mine[0].x, mine[1].x);
 #pragma unroll
-  for (int step = 1; step < 64; step *= 2) total += __shfl_xor(total, step);
+  for (int step = 1; step < 32; step *= 2) m = fmaxf(m, __shfl_xor(m, step));
+  float f[2], total = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    f[j] = lane + 32 * j >= a.splits ? 0.0f : mine[j].x == m ? 1.0f : __builtin_amdgcn_exp2f(mine[j].x - m);
+    total += f[j] * mine[j].y;
+  }
+#pragma unroll
+  for (int step = 1; step < 32; step *= 2) total += __shfl_xor(total, step);
   // Eight parts' loads at once; past the last part its own again, with a weight of 0.
-  float o[2] = {0.0f, 0.0f};
+  const int ch = min(4 * lane, a.head_dim - 4);
+  const float* from = a.partial + n * a.splits * a.head_dim + ch;
+  floatx4 o{};
   for (int k0 = 0; k0 < a.splits; k0 += 8) {
-    float x[8][2];
+    floatx4 x[8];
 #pragma unroll
     for (int k = 0; k < 8; k++)
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-        x[k][j] = from[(int64_t)min(k0 + k, a.splits - 1) * (a.head_dim + 2) + min(lane + 64 * j, a.head_dim - 1)];
+      x[k] = *reinterpret_cast<const floatx4*>(from + (int64_t)min(k0 + k, a.splits - 1) * a.head_dim);
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-      const float w = __shfl(f, k0 + k);
+      const float w = __shfl(k0 < 32 ? f[0] : f[1], (k0 + k) & 31, 32);
 #pragma unroll
-      for (int j = 0; j < 2; j++) o[j] += w * x[k][j];
+      for (int j = 0; j < 4; j++) o[j] += w * x[k][j];
     }
   }
   const bool live = i < s.queries && total != 0.0f;
-  T* to = reinterpret_cast<T*>(a.out + b * a.so.batch + i * a.so.token + h * a.so.head);
-#pragma unroll
-  for (int j = 0; j < 2; j++)
-    if (lane + 64 * j < a.head_dim) to[lane + 64 * j] = (T)(live ? o[j] / total : 0.0f);
+  if (4 * lane < a.head_dim) {
+    T* to = reinterpret_cast<T*>(a.out + b * a.so.batch + i * a.so.token + h * a.so.head) + ch;
+    put4(to, live ? o[0] / total : 0.0f, live ? o[1] / total : 0.0f, live ? o[2] / total : 0.0f,
+         live ? o[3] / total : 0.0f);
+  }
   if (lane == 0 && a.lse) a.lse[lse_index(a, b, h, i)] = live ? row_lse<T>(m, total) : -INFINITY;
 }
 
@@ -422,8 +439,6 @@ struct Plan {
   int parts;  // of a block of keys, in a workgroup: window_rows_kernel
   int tiles, splits;
 };
-
-constexpr int kMaxSplits = 64;  // a lane each in window_join_kernel
 
 Plan plan(const afhip_window_desc& d) {
   const bool f32 = d.dtype == AFHIP_F32;
@@ -491,8 +506,8 @@ template <typename T, int DP> int launch_forward(const WindowArgs& a, const Plan
   }
   if (s || p.splits == 1) return s;
   const int64_t rows = (int64_t)a.batch * a.queries * a.query_heads;
-  if ((s = check_grid(ceil_div(rows, 4), 256))) return s;
-  return launch("window.join", window_join_kernel<T>, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a);
+  if ((s = check_grid(ceil_div(rows, kJoinRows), 256))) return s;
+  return launch("window.join", window_join_kernel<T>, dim3((unsigned)ceil_div(rows, kJoinRows)), dim3(256), 0, st, a);
 }
 
 template <typename T> int launch_width(const WindowArgs& a, const Plan& p, hipStream_t st) {
