@@ -390,6 +390,64 @@ def test_what_is_not_seen_may_hold_anything(dtype, dev):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_what_lies_past_the_lengths_on_the_way_back(dtype, dev):
+    # out, its gradient and q hold NaN past the queries, k and v past the keys: the same bits as with zeros there.
+    import torch
+
+    from afhip import window
+
+    rng, dt = np.random.default_rng(24), torch_dtype(dtype)
+    for mask in (dict(left=30, sinks=2), dict(), dict(left=5, right=9)):
+        op = window.WindowAttention(4, 2, 64, dtype=dtype, **mask)
+        q, dout = (normal(rng, dev, dt, 2, 100, 4, 64) for _ in range(2))
+        k, v = (normal(rng, dev, dt, 2, 130, 2, 64) for _ in range(2))
+        ql, kl = ints([70, 100], dev), ints([130, 90], dev)
+        out, lse = op(q, k, v, query_lengths=ql, key_lengths=kl, return_lse=True)
+        want = op.backward(q, k, v, out, lse, dout, query_lengths=ql, key_lengths=kl)
+        for x in (q, dout, out):
+            x[0, 70:] = math.nan
+        for x in (k, v):
+            x[1, 90:] = math.nan
+        got = op.backward(q, k, v, out, lse, dout, query_lengths=ql, key_lengths=kl)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), mask
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_lengths_past_the_ends(dtype, dev):
+    # Below zero and past the tensors' ends they count as the nearer end.
+    import torch
+
+    from afhip import window
+
+    rng, dt = np.random.default_rng(25), torch_dtype(dtype)
+    op = window.WindowAttention(4, 2, 32, left=30, dtype=dtype)
+    q, dout = (normal(rng, dev, dt, 3, 60, 4, 32) for _ in range(2))
+    k, v = (normal(rng, dev, dt, 3, 80, 2, 32) for _ in range(2))
+
+    def both(ql, kl):
+        at = dict(query_lengths=ints(ql, dev), key_lengths=ints(kl, dev))
+        out, lse = op(q, k, v, return_lse=True, **at)
+        return out, lse, *op.backward(q, k, v, out, lse, dout, **at)
+
+    for a, b in zip(both([60, 0, 60], [80, 80, 0]), both([2 ** 31 - 1, -5, 61], [81, 2 ** 31 - 1, -2 ** 31])):
+        assert torch.equal(a, b)
+
+
+def test_f16_backward_of_large_scores(dev):
+    # Scores of +-60 and gradients that grow along the keys: ds' power of two falls again and again.
+    import torch
+
+    from afhip import window
+
+    rng, dt = np.random.default_rng(26), torch_dtype("f16")
+    op = window.WindowAttention(4, 2, 64, right=None, dtype="f16")
+    q, k = normal(rng, dev, dt, 1, 90, 4, 64, scale=4.0), normal(rng, dev, dt, 1, 700, 2, 64, scale=4.0)
+    v = normal(rng, dev, dt, 1, 700, 2, 64)
+    v *= torch.from_numpy(2.0 ** (np.arange(700) / 64.0)).to(dev).to(dt)[None, :, None, None]
+    compare(op, q, k, v, None, None, "f16", dev, None, None, 0, what="growing")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_large_and_equal_scores(dtype, dev):
     # Scores of +-500 (a probability that underflows counts as nothing), and equal ones (each probability 1 / n).
     from afhip import window
