@@ -53,20 +53,67 @@ struct RotaryArgs {
   float epsilon, turn;
 };
 
-template <typename T> struct Four;
-template <> struct Four<half_t> { typedef half4 type; };
-template <> struct Four<float> { typedef floatx4 type; };
-
-template <typename T> __device__ __forceinline__ void load4(const char* row, int channel, float* x) {
-  const auto v = *reinterpret_cast<const typename Four<T>::type*>(row + channel * sizeof(T));
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = (float)v[i];
+// The channels a lane has, of a row: four times two neighbours. Turned ones are four pairs, in the half layout two
+// fours; where rotary_dim is an odd multiple of 4 (ODD), the last of them has two pairs, and in the half layout the
+// four channels behind rotary_dim, two after its low and two after its high ones.
+struct Channels {
+  int first[4];
+};
+template <bool ODD> __device__ __forceinline__ Channels channels_of(int unit, int rotary_dim, bool half) {
+  const int pairs = rotary_dim / 2;
+  Channels c;
+  c.first[0] = half && 8 * unit < rotary_dim ? 4 * unit : 8 * unit;
+  c.first[2] = half && 8 * unit < rotary_dim ? pairs + 4 * unit : 8 * unit + 4;
+  const bool last = ODD && half && 8 * unit < rotary_dim && 8 * unit + 4 == rotary_dim;
+  c.first[1] = last ? rotary_dim : c.first[0] + 2;
+  c.first[3] = last ? rotary_dim + 2 : c.first[2] + 2;
+  return c;
 }
-template <typename T> __device__ __forceinline__ void store4(char* row, int channel, const float* x) {
-  typename Four<T>::type v;
+
+template <typename T> struct Vector;
+template <> struct Vector<half_t> {
+  typedef half4 four;
+  typedef half_t two __attribute__((ext_vector_type(2)));
+};
+template <> struct Vector<float> {
+  typedef floatx4 four;
+  typedef float two __attribute__((ext_vector_type(2)));
+};
+
+template <typename T, bool ODD> __device__ __forceinline__ void load8(const char* row, const Channels& c, float* x) {
+  const T* p = reinterpret_cast<const T*>(row);
+  if constexpr (ODD) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = (T)x[i];
-  *reinterpret_cast<typename Four<T>::type*>(row + channel * sizeof(T)) = v;
+    for (int i = 0; i < 8; i += 2) {
+      const auto v = *reinterpret_cast<const typename Vector<T>::two*>(p + c.first[i / 2]);
+      x[i] = (float)v[0];
+      x[i + 1] = (float)v[1];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const auto v = *reinterpret_cast<const typename Vector<T>::four*>(p + c.first[i / 2]);
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[i + j] = (float)v[j];
+    }
+  }
+}
+template <typename T, bool ODD> __device__ __forceinline__ void store8(char* row, const Channels& c, const float* x) {
+  T* p = reinterpret_cast<T*>(row);
+  if constexpr (ODD) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+      *reinterpret_cast<typename Vector<T>::two*>(p + c.first[i / 2]) =
+          typename Vector<T>::two{(T)x[i], (T)x[i + 1]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      typename Vector<T>::four v;
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = (T)x[i + j];
+      *reinterpret_cast<typename Vector<T>::four*>(p + c.first[i / 2]) = v;
+    }
+  }
 }
 
 // Sum over a row's lanes, each of them receiving it.
@@ -104,16 +151,16 @@ __device__ __forceinline__ void fill_turns(const RotaryArgs& a, int b, int first
   }
 }
 
-// Turns a lane's four pairs; sign -1 goes back.
-template <int SIGN> __device__ __forceinline__ void turn4(const float2* turns, bool half, float* x) {
+// Turns a lane's four pairs, or where `two` the first two of them; sign -1 goes back.
+template <int SIGN> __device__ __forceinline__ void turn4(const float2* turns, bool half, bool two, float* x) {
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     const float2 cs = turns[j];
     const float sn = SIGN * cs.y;
     float &x0 = half ? x[j] : x[2 * j], &x1 = half ? x[4 + j] : x[2 * j + 1];
     const float a = x0, b = x1;
-    x0 = a * cs.x - b * sn;
-    x1 = b * cs.x + a * sn;
+    x0 = two && j >= 2 ? a : a * cs.x - b * sn;
+    x1 = two && j >= 2 ? b : b * cs.x + a * sn;
   }
 }
 
@@ -144,7 +191,8 @@ __device__ __forceinline__ int pick_side(const RotaryArgs& a, int& group) {
   return 2;
 }
 
-template <typename T, int LANES, int NORM> __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
+template <typename T, int LANES, int NORM, bool ODD>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   constexpr int GROUPS = kThreads / LANES;
   __shared__ float2 turns[kMostTokens * kMaxHeadDim / 2];
   int tile;
@@ -158,7 +206,8 @@ template <typename T, int LANES, int NORM> __global__ __launch_bounds__(kThreads
   const int token = (int)s.sx.token;  // at most 2^24, of at most 16 tokens
   const int total = count * heads;
   const bool active = 8 * unit < D, turned = 8 * unit < a.rotary_dim, half = a.layout == AFHIP_ROTARY_HALF;
-  const int c0 = turned && half ? 4 * unit : 8 * unit, c1 = turned && half ? pairs + 4 * unit : 8 * unit + 4;
+  const bool two = ODD && 8 * unit + 4 == a.rotary_dim;
+  const Channels at = channels_of<ODD>(unit, a.rotary_dim, half);
   // A token past the length is read all the same, and not used. The first rows are on their way before all else.
   float x[kInFlight][8];
   auto load = [&](int n0) {
@@ -167,8 +216,7 @@ template <typename T, int LANES, int NORM> __global__ __launch_bounds__(kThreads
       const int n = min(n0 + r * GROUPS, total - 1), t = n / heads, h = n % heads;
       if (!active) continue;
       const char* p = from + t * token + h * s.sx.head;
-      load4<T>(p, c0, x[r]);
-      load4<T>(p, c1, x[r] + 4);
+      load8<T, ODD>(p, at, x[r]);
     }
   };
   if (!active) {
@@ -211,11 +259,9 @@ template <typename T, int LANES, int NORM> __global__ __launch_bounds__(kThreads
   }
   float w[8], c[8];
   if (NORM != AFHIP_HEAD_NORM_NONE && active) {
-    load4<float>(reinterpret_cast<const char*>(s.scale), c0, w);
-    load4<float>(reinterpret_cast<const char*>(s.scale), c1, w + 4);
+    load8<float, ODD>(reinterpret_cast<const char*>(s.scale), at, w);
     if (NORM == AFHIP_HEAD_NORM_LAYER) {
-      load4<float>(reinterpret_cast<const char*>(s.offset), c0, c);
-      load4<float>(reinterpret_cast<const char*>(s.offset), c1, c + 4);
+      load8<float, ODD>(reinterpret_cast<const char*>(s.offset), at, c);
     }
   }
   fill_turns(a, b, first, count, turns);
@@ -233,13 +279,12 @@ template <typename T, int LANES, int NORM> __global__ __launch_bounds__(kThreads
           if (NORM == AFHIP_HEAD_NORM_LAYER) x[r][j] += c[j];
         }
       }
-      if (turned) turn4<1>(turns + t * pairs + 4 * unit, half, x[r]);
+      if (turned) turn4<1>(turns + t * pairs + 4 * unit, half, two, x[r]);
       if (!active || !writes(t)) continue;
 #pragma unroll
       for (int j = 0; j < 8; j++) x[r][j] = first + t < live ? x[r][j] : 0.0f;
       char* p = to + t * s.so.token + h * s.so.head;
-      store4<T>(p, c0, x[r]);
-      store4<T>(p, c1, x[r] + 4);
+      store8<T, ODD>(p, at, x[r]);
     }
     n0 += kInFlight * GROUPS;
     if (n0 < total) load(n0);
@@ -249,7 +294,7 @@ template <typename T, int LANES, int NORM> __global__ __launch_bounds__(kThreads
 // The way back. A workgroup takes every groups-th tile of its side's tokens and
 // keeps its lanes' sums of the vectors' gradients in registers until the end:
 // a row of partial sums each, which rotary_sums_kernel adds up.
-template <typename T, int LANES, int NORM>
+template <typename T, int LANES, int NORM, bool ODD>
 __global__ __launch_bounds__(kThreads) void rotary_backward_kernel(RotaryArgs a) {
   constexpr int GROUPS = kThreads / LANES, ROWS = 2;
   constexpr int VECTORS = NORM == AFHIP_HEAD_NORM_LAYER ? 2 : NORM == AFHIP_HEAD_NORM_RMS ? 1 : 0;
@@ -259,13 +304,11 @@ __global__ __launch_bounds__(kThreads) void rotary_backward_kernel(RotaryArgs a)
   const int unit = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int D = a.head_dim, pairs = a.rotary_dim / 2, heads = s.heads;
   const bool active = 8 * unit < D, turned = 8 * unit < a.rotary_dim, half = a.layout == AFHIP_ROTARY_HALF;
-  const int c0 = turned && half ? 4 * unit : 8 * unit, c1 = turned && half ? pairs + 4 * unit : 8 * unit + 4;
+  const bool two = ODD && 8 * unit + 4 == a.rotary_dim;
+  const Channels at = channels_of<ODD>(unit, a.rotary_dim, half);
   const float per = 1.0f / (float)D;
   float w[8], sums[VECTORS ? VECTORS : 1][8] = {};
-  if (VECTORS && active) {
-    load4<float>(reinterpret_cast<const char*>(s.scale), c0, w);
-    load4<float>(reinterpret_cast<const char*>(s.scale), c1, w + 4);
-  }
+  if (VECTORS && active) load8<float, ODD>(reinterpret_cast<const char*>(s.scale), at, w);
   for (int tile = mine; tile < a.batch * s.tiles; tile += s.groups) {
     const int b = tile / s.tiles, first = (tile % s.tiles) * s.tile_tokens;
     const int count = min(s.tile_tokens, a.tokens - first), total = count * heads;
@@ -287,12 +330,10 @@ __global__ __launch_bounds__(kThreads) void rotary_backward_kernel(RotaryArgs a)
         for (int j = 0; j < 8; j++) x[r][j] = g[r][j] = 0.0f;
         if (!active) continue;
         const char* p = gs + t * token_g + h * s.sg.head;
-        load4<T>(p, c0, g[r]);
-        load4<T>(p, c1, g[r] + 4);
+        load8<T, ODD>(p, at, g[r]);
         if constexpr (VECTORS != 0) {
           p = xs + t * token_x + h * s.sx.head;
-          load4<T>(p, c0, x[r]);
-          load4<T>(p, c1, x[r] + 4);
+          load8<T, ODD>(p, at, x[r]);
         }
       }
 #pragma unroll
@@ -300,7 +341,7 @@ __global__ __launch_bounds__(kThreads) void rotary_backward_kernel(RotaryArgs a)
         const int n = n0 + r * GROUPS, t = n / heads, h = n % heads;
         if (n >= total) break;
         const bool counts = active && first + t < live;
-        if (turned) turn4<-1>(turns + t * pairs + 4 * unit, half, g[r]);
+        if (turned) turn4<-1>(turns + t * pairs + 4 * unit, half, two, g[r]);
         if constexpr (VECTORS != 0) {
           const float root = normalize<LANES, NORM>(x[r], active, D, a.epsilon);
           float gx[8];
@@ -320,8 +361,7 @@ __global__ __launch_bounds__(kThreads) void rotary_backward_kernel(RotaryArgs a)
         for (int j = 0; j < 8; j++) g[r][j] = counts ? g[r][j] : 0.0f;
         if (!active) continue;
         char* p = to + (t * heads + h) * D * (int)sizeof(T);
-        store4<T>(p, c0, g[r]);
-        store4<T>(p, c1, g[r] + 4);
+        store8<T, ODD>(p, at, g[r]);
       }
     }
   }
@@ -335,7 +375,7 @@ __global__ __launch_bounds__(kThreads) void rotary_backward_kernel(RotaryArgs a)
         float y = sums[v][j];
 #pragma unroll
         for (int step = LANES; step < 64; step *= 2) y += __shfl_xor(y, step);
-        if (active && (threadIdx.x & 63) < LANES) rows[wave][v][j < 4 ? c0 + j : c1 + j - 4] = y;
+        if (active && (threadIdx.x & 63) < LANES) rows[wave][v][at.first[j / 2] + j % 2] = y;
       }
     }
     __syncthreads();
@@ -378,8 +418,8 @@ int check(const afhip_rotary_desc* desc) {
                 "rotary dimensions must be positive");
   AFHIP_REQUIRE(d.head_dim % 8 == 0 && d.head_dim <= kMaxHeadDim, "head dimension %d is not a multiple of 8 up to %d",
                 d.head_dim, kMaxHeadDim);
-  AFHIP_REQUIRE(d.rotary_dim >= 0 && d.rotary_dim % 8 == 0 && d.rotary_dim <= d.head_dim,
-                "rotary dimension %d is not a multiple of 8 up to the head dimension %d", d.rotary_dim, d.head_dim);
+  AFHIP_REQUIRE(d.rotary_dim >= 0 && d.rotary_dim % 4 == 0 && d.rotary_dim <= d.head_dim,
+                "rotary dimension %d is not a multiple of 4 up to the head dimension %d", d.rotary_dim, d.head_dim);
   AFHIP_REQUIRE(d.query_heads <= 65536 && d.key_heads <= 65536, "more than 65,536 heads");
   AFHIP_REQUIRE(d.layout == AFHIP_ROTARY_HALF || d.layout == AFHIP_ROTARY_INTERLEAVED, "unknown rotary layout %d",
                 d.layout);
@@ -441,23 +481,30 @@ RotaryArgs fill(const afhip_rotary_desc& d, const int32_t* past, const int32_t* 
   return a;
 }
 
-template <typename T, int LANES, int NORM> int launch_way(const RotaryArgs& a, bool back, hipStream_t st) {
+template <typename T, int LANES, int NORM, bool ODD> int launch_way(const RotaryArgs& a, bool back, hipStream_t st) {
   const int64_t groups = (int64_t)a.side[0].groups + a.side[1].groups + a.side[2].groups;
   if (int s = check_grid(groups, kThreads)) return s;
   const dim3 grid((unsigned)groups);
   if (back)
-    return launch("rotary.backward", rotary_backward_kernel<T, LANES, NORM>, grid, dim3(kThreads), 0, st, a);
-  return launch("rotary", rotary_kernel<T, LANES, NORM>, grid, dim3(kThreads), 0, st, a);
+    return launch("rotary.backward", rotary_backward_kernel<T, LANES, NORM, ODD>, grid, dim3(kThreads), 0, st, a);
+  return launch("rotary", rotary_kernel<T, LANES, NORM, ODD>, grid, dim3(kThreads), 0, st, a);
+}
+
+template <typename T, int LANES, int NORM> int launch_odd(const RotaryArgs& a, bool back, hipStream_t st) {
+  if constexpr (LANES > 1)
+    if (a.rotary_dim % 8) return launch_way<T, LANES, NORM, true>(a, back, st);
+  return launch_way<T, LANES, NORM, false>(a, back, st);
 }
 
 template <typename T, int LANES> int launch_norm(const RotaryArgs& a, int norm, bool back, hipStream_t st) {
-  if (norm == AFHIP_HEAD_NORM_NONE) return launch_way<T, LANES, AFHIP_HEAD_NORM_NONE>(a, back, st);
-  if (norm == AFHIP_HEAD_NORM_RMS) return launch_way<T, LANES, AFHIP_HEAD_NORM_RMS>(a, back, st);
-  return launch_way<T, LANES, AFHIP_HEAD_NORM_LAYER>(a, back, st);
+  if (norm == AFHIP_HEAD_NORM_NONE) return launch_odd<T, LANES, AFHIP_HEAD_NORM_NONE>(a, back, st);
+  if (norm == AFHIP_HEAD_NORM_RMS) return launch_odd<T, LANES, AFHIP_HEAD_NORM_RMS>(a, back, st);
+  return launch_odd<T, LANES, AFHIP_HEAD_NORM_LAYER>(a, back, st);
 }
 
 template <typename T> int launch_lanes(const RotaryArgs& a, int norm, bool back, hipStream_t st) {
-  if (a.head_dim <= 8) return launch_norm<T, 1>(a, norm, back, st);
+  // 4 turned channels of 8 take two lanes: where all lanes have the same channels scalar registers hold them, too many.
+  if (a.head_dim <= 8 && a.rotary_dim % 8 == 0) return launch_norm<T, 1>(a, norm, back, st);
   if (a.head_dim <= 16) return launch_norm<T, 2>(a, norm, back, st);
   if (a.head_dim <= 32) return launch_norm<T, 4>(a, norm, back, st);
   if (a.head_dim <= 64) return launch_norm<T, 8>(a, norm, back, st);

@@ -496,7 +496,7 @@ typedef struct afhip_rotary_desc {
   int32_t batch, tokens;
   int32_t query_heads, key_heads;
   int32_t head_dim;   /* a multiple of 8, at most 128 */
-  int32_t rotary_dim; /* a multiple of 8, at most head_dim; 0 turns nothing */
+  int32_t rotary_dim; /* a multiple of 4, at most head_dim; 0 turns nothing */
   int32_t layout;     /* AFHIP_ROTARY_* */
   int32_t norm;       /* AFHIP_HEAD_NORM_* */
   int32_t dtype;      /* of every tensor with channels: AFHIP_F32 | AFHIP_F16 */

@@ -92,6 +92,13 @@ CASES = [
     (2, 1500, 3, 1, 128, 64, "interleaved", "layer", "f16"),
     (1, 4, 2, 2, 64, 0, "half", "rms", "f32"),
     (70, 1, 16, 2, 24, 24, "interleaved", None, "f16"),
+    # Odd multiples of 4: the last pairs share a lane with channels that do not turn.
+    (2, 37, 6, 3, 40, 20, "half", "rms", "f16"),
+    (1, 45, 8, 2, 40, 20, "interleaved", "layer", "f32"),
+    (2, 19, 3, 1, 8, 4, "half", "layer", "f32"),
+    (1, 90, 4, 2, 128, 100, "half", "layer", "f16"),
+    (3, 11, 2, 2, 128, 124, "interleaved", "rms", "f32"),
+    (2, 21, 4, 4, 80, 76, "half", None, "f32"),
 ]
 
 
@@ -393,7 +400,7 @@ def test_refusals(dev):
                      key_offset=np.ones(32, np.float32))):
         with pytest.raises(_lib.RangeError):
             fresh.prepare(**bad)
-    for bad in (dict(dtype="bf16"), dict(layout="other"), dict(norm="batch"), dict(rotary_dim=12),
+    for bad in (dict(dtype="bf16"), dict(layout="other"), dict(norm="batch"), dict(rotary_dim=10),
                 dict(frequencies=np.ones(3))):
         with pytest.raises(_lib.RangeError):
             rotary.HeadRotary(4, 2, 32, **{"dtype": "f16", **bad})

@@ -65,7 +65,7 @@ def test_window_refusals(change, message):
 @pytest.mark.parametrize("change, message", [
     (dict(batch=0), "positive"), (dict(tokens=-1), "positive"), (dict(key_heads=0), "positive"),
     (dict(head_dim=20), "multiple of 8"), (dict(head_dim=256), "multiple of 8"),
-    (dict(rotary_dim=12), "multiple of 8"), (dict(rotary_dim=72), "multiple of 8"), (dict(rotary_dim=-8), "multiple"),
+    (dict(rotary_dim=10), "multiple of 4"), (dict(rotary_dim=72), "multiple of 4"), (dict(rotary_dim=-8), "multiple"),
     (dict(layout=2), "layout"), (dict(norm=3), "norm"), (dict(dtype=2), "f32 or f16"), (dict(capacity=-1), "capacity"),
     (dict(epsilon=-1.0), "epsilon"), (dict(epsilon=math.nan), "epsilon"), (dict(rotation_scale=math.inf), "finite"),
     (dict(batch=1 << 20, tokens=1 << 10), "2\\^29"), (dict(q=(5 * 256, 256, 4)), "16 bytes"),
