@@ -148,6 +148,45 @@ template <typename T, int DP> struct Tile {
   }
 };
 
+// The same tile of ROWS rows of f32 as three of bf16, one behind the other, made once a workgroup by split_two.
+template <int DP, int ROWS> struct Planes {
+  typedef Tile<half_t, DP> Half;
+  static constexpr int kPlane = ROWS * Half::kRow, kBytes = 3 * kPlane;
+
+  static __device__ __forceinline__ Parts8 nat(const unsigned char* t, int row, int kk, int hi) {
+    Parts8 p;
+    p.high = __builtin_bit_cast(bf16x8, Half::nat(t, row, kk, hi));
+    p.mid = __builtin_bit_cast(bf16x8, Half::nat(t + kPlane, row, kk, hi));
+    p.low = __builtin_bit_cast(bf16x8, Half::nat(t + 2 * kPlane, row, kk, hi));
+    return p;
+  }
+  static __device__ __forceinline__ Parts8 tr(const unsigned char* t, int row0, int cb, int lane) {
+    Parts8 p;
+    p.high = __builtin_bit_cast(bf16x8, Half::tr(t, row0, cb, lane));
+    p.mid = __builtin_bit_cast(bf16x8, Half::tr(t + kPlane, row0, cb, lane));
+    p.low = __builtin_bit_cast(bf16x8, Half::tr(t + 2 * kPlane, row0, cb, lane));
+    return p;
+  }
+  // Of two tiles, one behind the other, eight channels of a row at a time, by THREADS threads.
+  template <int THREADS> static __device__ __forceinline__ void split_two(const unsigned char* raw, unsigned char* t) {
+    constexpr int EIGHTS = DP / 8, RAW = Tile<float, DP>::kRow;
+    static_assert(2 * ROWS * EIGHTS % THREADS == 0, "as many for each thread");
+#pragma unroll 2
+    for (int n = threadIdx.x; n < 2 * ROWS * EIGHTS; n += THREADS) {
+      const int r = n / EIGHTS, e = n % EIGHTS, which = r / ROWS, row = r % ROWS;
+      const unsigned char* from = raw + r * RAW;
+      const int sw = Tile<float, DP>::swizzle(row);
+      const floatx4 a = *reinterpret_cast<const floatx4*>(from + 16 * ((2 * e) ^ sw));
+      const floatx4 b = *reinterpret_cast<const floatx4*>(from + 16 * ((2 * e + 1) ^ sw));
+      const Parts8 p = split_parts(floatx8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+      unsigned char* to = t + which * kBytes + row * Half::kRow + 16 * (e ^ Half::swizzle(row));
+      *reinterpret_cast<bf16x8*>(to) = p.high;
+      *reinterpret_cast<bf16x8*>(to + kPlane) = p.mid;
+      *reinterpret_cast<bf16x8*>(to + 2 * kPlane) = p.low;
+    }
+  }
+};
+
 // What a wave loads of a tile of ROWS rows of a tensor, shared among WAVES waves.
 template <typename T, int DP, int ROWS, int WAVES> struct TileLoad {
   static constexpr int kChunks = Tile<T, DP>::kChunks, kCount = ROWS * kChunks / 64 / WAVES;

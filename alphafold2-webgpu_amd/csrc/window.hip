@@ -21,6 +21,7 @@
 // and the comparisons run only in blocks that some row sees in part.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "window.h"
 
@@ -62,7 +63,7 @@ template <typename T, int DP> struct Rows {
   }
 
   // 32 NB keys from k0 on: K and V tiles at kt and vt; ends and starts: see hide().
-  template <int NB>
+  template <typename Read, int NB>
   __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int k0, bool ends, bool starts,
                                        int sinks, float scale, int lane) {
     const int col = lane & 31, hi = lane >> 5;
@@ -71,7 +72,7 @@ template <typename T, int DP> struct Rows {
     for (int n = 0; n < NB; n++) {
       x[n] = floatx16{};
 #pragma unroll
-      for (int kk = 0; kk < kSteps; kk++) x[n] = mma(Tile<T, DP>::nat(kt, 32 * n + col, kk, hi), q[kk], x[n]);
+      for (int kk = 0; kk < kSteps; kk++) x[n] = mma(Read::nat(kt, 32 * n + col, kk, hi), q[kk], x[n]);
     }
     if (ends | starts) {
 #pragma unroll
@@ -106,7 +107,7 @@ template <typename T, int DP> struct Rows {
       for (int s = 0; s < 2; s++) {
         const Frag f = pack8(p + 8 * s, (Frag*)nullptr);
 #pragma unroll
-        for (int c = 0; c < kBlocks; c++) o[c] = mma(Tile<T, DP>::tr(vt, 32 * n + 16 * s, c, lane), f, o[c]);
+        for (int c = 0; c < kBlocks; c++) o[c] = mma(Read::tr(vt, 32 * n + 16 * s, c, lane), f, o[c]);
       }
     }
   }
@@ -135,7 +136,9 @@ __device__ __forceinline__ float2* part_totals(const WindowArgs& a) {
 // window 1,024 over 16,384 tokens, 8 heads over 2, 87 us.
 constexpr int kWaves = 4, kTileRows = 32 * kWaves;
 template <typename T> constexpr int kBlockKeys = sizeof(T) == 2 ? 64 : 32;  // a wave's, of a block
-template <typename T, int DP, int PARTS> constexpr int kRowsLds = 4 * PARTS * kBlockKeys<T> * DP * (int)sizeof(T);
+// f32 blocks are loaded into one buffer and made three bf16 from there, once for all waves.
+template <typename T, int DP, int PARTS>
+constexpr int kRowsLds = (sizeof(T) == 2 ? 8 : 20) * PARTS * kBlockKeys<T> * DP;
 // f32 over 128 channels takes more than the 256 registers that eight waves have each.
 template <typename T, int DP> constexpr bool kTwoParts = DP * sizeof(T) <= 256;
 
@@ -143,7 +146,10 @@ template <typename T, int DP, bool SPLIT, int PARTS>
 __global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) > 256 ? 1 : 2) void window_rows_kernel(
     WindowArgs a) {
   constexpr int WK = kBlockKeys<T>, BK = WK * PARTS;
+  constexpr bool F32 = sizeof(T) == 4;
   typedef TileLoad<T, DP, BK, kWaves * PARTS> Load;
+  typedef Planes<DP, BK> Split;
+  typedef typename std::conditional<F32, Split, Tile<T, DP>>::type Read;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   prefer_one_of_two();
   const int lane = threadIdx.x & 63, hi = lane >> 5;
@@ -175,7 +181,7 @@ __global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) >
   vload.init(wave, lane, a.head_dim, a.sv.token);
   auto issue = [&](int t) {
     const int k0 = range.block(t) * BK;
-    const uint32_t buffer = lds + (uint32_t)((t - begin) & 1) * 2 * Load::kBytes;
+    const uint32_t buffer = lds + (F32 ? 0u : (uint32_t)((t - begin) & 1) * 2 * Load::kBytes);
     const bool whole = range.whole(k0, BK);
     auto keep = [&](int key) { return range.keeps(key); };
     kload.issue(kb, a.sk.token, k0, buffer, wave, whole, keep);
@@ -185,6 +191,10 @@ __global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) >
   auto arrive = [&](int t) {
     wait_vmcnt<0>();
     block_barrier();
+    if constexpr (F32) {
+      Split::template split_two<64 * kWaves * PARTS>(smem, smem + 2 * Load::kBytes);
+      block_barrier();  // written, and the buffer is read
+    }
     if (t + 1 < end) issue(t + 1);
   };
   // The first keys are on their way before the queries.
@@ -201,8 +211,10 @@ __global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) >
     for (; t < work; t++) {
       arrive(t);
       const int at = WK * part, k0 = range.block(t) * BK + at;
-      const unsigned char* kt = smem + ((t - begin) & 1) * 2 * Load::kBytes + at * Tile<T, DP>::kRow;
-      st.template step<WK / 32>(kt, kt + Load::kBytes, k0, k0 + WK > all_high, k0 < all_low && k0 + WK > range.sinks,
+      const unsigned char* kt = F32 ? smem + 2 * Load::kBytes + at * DP * 2
+                                    : smem + ((t - begin) & 1) * 2 * Load::kBytes + at * DP * 2;
+      const unsigned char* vt = kt + (F32 ? Split::kBytes : Load::kBytes);
+      st.template step<Read, WK / 32>(kt, vt, k0, k0 + WK > all_high, k0 < all_low && k0 + WK > range.sinks,
                                 range.sinks, a.scale_log2, lane);
     }
     for (; t < idle; t++) arrive(t);
@@ -336,7 +348,7 @@ __global__ __launch_bounds__((kStepThreads<T, DP>)) void window_step_kernel(Wind
     }
     const int k0 = range.block(begin + wave + n * W) * 32;
     const unsigned char* kt = smem + (wave * STAGES + n % STAGES) * S::kBytes;
-    st.template step<1>(kt, kt + S::kBytes / 2, k0, k0 + 32 > all_high, k0 < all_low && k0 + 32 > range.sinks,
+    st.template step<Tile<T, DP>, 1>(kt, kt + S::kBytes / 2, k0, k0 + 32 > all_high, k0 < all_low && k0 + 32 > range.sinks,
                         range.sinks, a.scale_log2, lane);
   }
   // The waves' reference points, totals and sums: [wave][row][m, l, DP sums].
