@@ -171,7 +171,7 @@ template <int DP, int ROWS> struct Planes {
   template <int THREADS> static __device__ __forceinline__ void split_two(const unsigned char* raw, unsigned char* t) {
     constexpr int EIGHTS = DP / 8, RAW = Tile<float, DP>::kRow;
     static_assert(2 * ROWS * EIGHTS % THREADS == 0, "as many for each thread");
-#pragma unroll 2
+#pragma unroll 1
     for (int n = threadIdx.x; n < 2 * ROWS * EIGHTS; n += THREADS) {
       const int r = n / EIGHTS, e = n % EIGHTS, which = r / ROWS, row = r % ROWS;
       const unsigned char* from = raw + r * RAW;
@@ -194,8 +194,8 @@ template <typename T, int DP, int ROWS, int WAVES> struct TileLoad {
   static_assert(ROWS * kChunks % (64 * WAVES) == 0, "whole instructions for each wave");
 
   static constexpr int kStep = 64 / kChunks;  // rows of an instruction
-  // Offsets held for whole tiles, where they are few.
-  static constexpr bool kHeld = kCount <= 4;
+  // Offsets held for whole tiles, where they are few and registers are not.
+  static constexpr bool kHeld = kCount <= 4 && DP * sizeof(T) <= 256;
   static constexpr int kUnroll = kHeld ? kCount : 2;
   int row, chunk, chunks;  // the lane's row and chunk in a wave's first instruction; a row's chunks
   uint32_t held[kHeld ? kCount : 1];

@@ -34,6 +34,12 @@ namespace {
 template <typename T> constexpr float kLift = sizeof(T) == 2 ? 6.0f : 0.0f;
 constexpr float kSlack = 8.0f;
 
+// f32 over 128 channels just fits the 256 registers that each of eight waves has, where no fragments are read far
+// ahead: two workgroups of four waves a CU. 2,000 tokens, 32 heads over 8, in 500 workgroups, us, two / one a CU: no
+// mask 347 / 430, window 300 71 / 97; but 352 workgroups, causal, 97 / 86, since a CU gets its second before others
+// have one.
+template <typename T, int DP> constexpr bool kWide = DP * sizeof(T) > 256;
+
 // One wave's 32 rows: Q, the running state and the output so far.
 template <typename T, int DP> struct Rows {
   typedef typename Eight<T>::type Frag;
@@ -72,7 +78,10 @@ template <typename T, int DP> struct Rows {
     for (int n = 0; n < NB; n++) {
       x[n] = floatx16{};
 #pragma unroll
-      for (int kk = 0; kk < kSteps; kk++) x[n] = mma(Read::nat(kt, 32 * n + col, kk, hi), q[kk], x[n]);
+      for (int kk = 0; kk < kSteps; kk++) {
+        x[n] = mma(Read::nat(kt, 32 * n + col, kk, hi), q[kk], x[n]);
+        if (kWide<T, DP> && kk % 2) __builtin_amdgcn_sched_barrier(0);
+      }
     }
     if (ends | starts) {
 #pragma unroll
@@ -107,7 +116,10 @@ template <typename T, int DP> struct Rows {
       for (int s = 0; s < 2; s++) {
         const Frag f = pack8(p + 8 * s, (Frag*)nullptr);
 #pragma unroll
-        for (int c = 0; c < kBlocks; c++) o[c] = mma(Read::tr(vt, 32 * n + 16 * s, c, lane), f, o[c]);
+        for (int c = 0; c < kBlocks; c++) {
+          o[c] = mma(Read::tr(vt, 32 * n + 16 * s, c, lane), f, o[c]);
+          if (kWide<T, DP>) __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   }
@@ -139,11 +151,9 @@ template <typename T> constexpr int kBlockKeys = sizeof(T) == 2 ? 64 : 32;  // a
 // f32 blocks are loaded into one buffer and made three bf16 from there, once for all waves.
 template <typename T, int DP, int PARTS>
 constexpr int kRowsLds = (sizeof(T) == 2 ? 8 : 20) * PARTS * kBlockKeys<T> * DP;
-// f32 over 128 channels takes more than the 256 registers that eight waves have each.
-template <typename T, int DP> constexpr bool kTwoParts = DP * sizeof(T) <= 256;
 
 template <typename T, int DP, bool SPLIT, int PARTS>
-__global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) > 256 ? 1 : 2) void window_rows_kernel(
+__global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 ? 1 : 2) void window_rows_kernel(
     WindowArgs a) {
   constexpr int WK = kBlockKeys<T>, BK = WK * PARTS;
   constexpr bool F32 = sizeof(T) == 4;
@@ -159,10 +169,13 @@ __global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) >
   const int heads = a.batch * a.key_heads;
   const int pair = blockIdx.x % heads, rest = blockIdx.x / heads;
   const int b = pair / a.key_heads, kv = pair % a.key_heads;
-  const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
+  const int turn = rest % a.tiles, split = rest / a.tiles, half = (a.tiles + 1) / 2;
+  // Where all run at once, two a CU, the second ones from the shortest on.
+  const bool second = kWide<T, DP> && gridDim.x <= 512 && (SPLIT ? 2 * split >= a.splits : turn >= half);
+  const int tile = second ? (SPLIT ? turn : turn - half) : a.tiles - 1 - turn;
   const Sequence s(a, b);
   const int rows = a.queries * a.group;
-  const int r0 = tile * kTileRows, row = r0 + 32 * rg + (lane & 31);
+  const int r0 = tile * kTileRows;
   const int first = r0 / a.group, last = min(s.queries - 1, (r0 + kTileRows - 1) / a.group);
 
   const KeyRange range(a, s, first, last, BK);
@@ -200,7 +213,7 @@ __global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) >
   // The first keys are on their way before the queries.
   if (begin < end) issue(begin);
   Rows<T, DP> st;
-  st.init(a, s, b, kv, row, hi);
+  st.init(a, s, b, kv, r0 + 32 * rg + (lane & 31), hi);
   // Blocks that the wave's rows see, between such that only other waves' do. (A branch around the work of one loop
   // would have the compiler copy all sums at its end.)
   const auto phases = range.phases(begin, end, BK, s.low(a, wfirst), s.high(a, wlast), wr0 < s.queries * a.group);
@@ -245,6 +258,9 @@ __global__ __launch_bounds__(64 * kWaves * PARTS, PARTS == 2 || DP * sizeof(T) >
       for (int v = 0; v < 16; v++) st.o[c][v] = st.o[c][v] * f + shared[(2 + 16 * c + v) * 64] * g;
   }
   const float l = st.l + __shfl_xor(st.l, 32);
+  int row = threadIdx.x;
+  asm volatile("" : "+v"(row));  // computed here, not held from the start
+  row = r0 + 32 * rg + (row & 31);
   if (row >= rows) return;
   const int i = row / a.group, h = kv * a.group + row % a.group;
   if constexpr (SPLIT) {
@@ -348,8 +364,8 @@ __global__ __launch_bounds__((kStepThreads<T, DP>)) void window_step_kernel(Wind
     }
     const int k0 = range.block(begin + wave + n * W) * 32;
     const unsigned char* kt = smem + (wave * STAGES + n % STAGES) * S::kBytes;
-    st.template step<Tile<T, DP>, 1>(kt, kt + S::kBytes / 2, k0, k0 + 32 > all_high, k0 < all_low && k0 + 32 > range.sinks,
-                        range.sinks, a.scale_log2, lane);
+    st.template step<Tile<T, DP>, 1>(kt, kt + S::kBytes / 2, k0, k0 + 32 > all_high,
+                                     k0 < all_low && k0 + 32 > range.sinks, range.sinks, a.scale_log2, lane);
   }
   // The waves' reference points, totals and sums: [wave][row][m, l, DP sums].
   float* sums = reinterpret_cast<float*>(smem);
@@ -458,7 +474,8 @@ Plan plan(const afhip_window_desc& d) {
   Plan p{};
   // Tiles of 32 rows also where those of 128 are few. Whole calls on MI355X, tiles of 128 / 32, us: f32 over 32
   // channels 128 tiles 15.9 / 10.1, 256 tiles 17.8 / 32; over 64 40 tiles 28 / 20, 64 tiles 35 / 37; over 128 40 tiles
-  // 33 / 34, 112 tiles 33 / 43; f16 over 64 channels 2 tiles 10.5 / 8.9, 128 tiles 12.7 / 16.5; over 128 20 tiles 12.2 / 13.6.
+  // 33 / 34, 112 tiles 33 / 43; f16 over 64 channels 2 tiles 10.5 / 8.9, 128 tiles 12.7 / 16.5; over 128 20 tiles
+  // 12.2 / 13.6.
   const int64_t few = f32 ? (d.head_dim <= 32 ? 256 : 64) : d.head_dim <= 64 ? 64 : 0;
   p.step = rows <= 32 || heads * ceil_div(rows, kTileRows) < few;
   p.tiles = (int)ceil_div(rows, p.step ? 32 : kTileRows);
@@ -473,9 +490,9 @@ Plan plan(const afhip_window_desc& d) {
     span = std::min(span, (int64_t)d.left + right + queries + std::min<int64_t>(d.sinks, d.keys));
   }
   // Into how many parts the keys are split: the shortest of some, by what they take on MI355X in us. A block of 32 keys
-  // takes a workgroup 0.4 (f16, 128 channels; f32 2.6, of four waves with keys of their own 1.2), a workgroup's start and end 4, a CU having one of them at a
-  // time; the keys' bytes come at 5.3 TB/s where all CUs ask for them, at 4 where half do; the join takes 4.5, and its
-  // sums go out and in at 3.5 TB/s.
+  // takes a workgroup 0.4 (f16, 128 channels; f32 2.6, of four waves with keys of their own 1.2), a workgroup's start
+  // and end 4, a CU having one of them at a time; the keys' bytes come at 5.3 TB/s where all CUs ask for them, at 4
+  // where half do; the join takes 4.5, and its sums go out and in at 3.5 TB/s.
   const double block = std::max((!f32 ? 0.4 : p.step ? 1.2 : 2.6) * d.head_dim / 128, 0.15);
   const double bytes = 2.0 * heads * span * d.head_dim * dtype_size(d.dtype);
   double best = INFINITY;
@@ -497,7 +514,8 @@ size_t partial_bytes(const afhip_window_desc& d, const Plan& p) {
 
 template <typename T, int DP, int PARTS>
 int launch_rows(const WindowArgs& a, const Plan& p, int64_t groups, hipStream_t st) {
-  constexpr size_t lds = kRowsLds<T, DP, PARTS>;
+  // Half of the LDS and more: one a CU.
+  const size_t lds = kRowsLds<T, DP, PARTS> + (kWide<T, DP> && groups < 448 ? 1024 : 0);
   auto k = p.splits > 1 ? window_rows_kernel<T, DP, true, PARTS> : window_rows_kernel<T, DP, false, PARTS>;
   int s;
   if ((s = check_grid(groups, 64 * kWaves * PARTS)) || (s = allow_lds((const void*)k, lds))) return s;
@@ -513,7 +531,7 @@ template <typename T, int DP> int launch_forward(const WindowArgs& a, const Plan
     if ((s = check_grid(groups, 64 * S::kWaves)) || (s = allow_lds((const void*)k, S::kLds))) return s;
     s = launch("window.step", k, dim3((unsigned)groups), dim3(64 * S::kWaves), S::kLds, st, a);
   } else {
-    s = p.parts == 2 ? launch_rows<T, DP, kTwoParts<T, DP> ? 2 : 1>(a, p, groups, st)
+    s = p.parts == 2 ? launch_rows<T, DP, kWide<T, DP> ? 1 : 2>(a, p, groups, st)
                      : launch_rows<T, DP, 1>(a, p, groups, st);
   }
   if (s || p.splits == 1) return s;
