@@ -275,7 +275,8 @@ __device__ __forceinline__ void put4(float* p, float a, float b, float c, float 
 }
 
 // Of two waves on a SIMD one goes first wherever both could issue, so that its MFMAs run beside the other's vector
-// instructions and not in step with them: the waves' slots tell them apart.
+// instructions and not in step with them: the waves' slots tell them apart. (dk and dv of 4,096 tokens, 16 heads over
+// 4 of 128 channels, window 1,024, f16: 97.0 us, and 99.2 without.)
 __device__ __forceinline__ void prefer_one_of_two() {
   constexpr int kWaveSlot = 4 | (0 << 6) | (3 << 11);  // HW_ID, bits 0 to 3
   if (__builtin_amdgcn_s_getreg(kWaveSlot) & 1) __builtin_amdgcn_s_setprio(1);

@@ -313,6 +313,7 @@ __global__ __launch_bounds__((kKeyTileThreads<T, DP>)) void window_dkv_kernel(Wi
   constexpr bool F16 = sizeof(T) == 2;
   constexpr float LIFT = F16 ? 13.0f : 0.0f;  // on P's exponent, and so on ds
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  prefer_one_of_two();
   const int lane = threadIdx.x & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wave % KT::kKeyGroups, rg = wave / KT::kKeyGroups;
